@@ -547,6 +547,139 @@ ngp_status ngp_accumulate_tonemap(const float* frame, float* accum, float* out, 
                                   uint32_t sample_count, int color_space, float exposure,
                                   const float* background_rgba, int output_srgb, ngp_stream stream);
 
+/* --- layers of any width -------------------------------------------------------------- */
+/* The parts of networks whose shape the fused MLPs above do not have (tcnn's CutlassMLP serves them upstream, the
+ * network object of src/testbed.cu:3726-3727): linear layers with bias, activation and residual, layer norm, and the
+ * activations a backward pass needs kept in 8 bits.  No model handle: every call works on the caller's device memory on
+ * `stream` (of the current device, or of the stream's own device), allocates nothing, never waits for the device and
+ * may be captured into a graph; what a call reads and writes must live until the stream has passed it.
+ *  - Matrices are row-major, strides in elements, at least the width and below 2^22; widths are 1..65536, rows 0..2^31-1.
+ *    Rows that start on 16 bytes (16-byte aligned pointers, strides that are multiples of 8 elements) and widths that are
+ *    multiples of 8 run in place; other layers' matrices are first copied into the workspace.
+ *  - Outputs must not overlap inputs or each other, except: y may be residual, dx may be dx_add (the same rows).
+ *  - Workspaces: the matching *_workspace call says how many bytes the same arguments need (0: none); 16-byte aligned,
+ *    owned by one call at a time (two streams or captured graphs that may run together need one each).
+ *  - Sums, means and statistics are held in fp32; sums over rows are taken in a fixed order (the same result every time).
+ *  - Non-finite values follow the formulas. */
+enum { NGP_TYPE_F32 = 0, NGP_TYPE_F16 = 1, NGP_TYPE_BF16 = 2 };
+enum {
+	NGP_ACT_NONE = 0, /* 0..3 as ENerfActivation (common.h:90-95) */
+	NGP_ACT_RELU = 1,
+	NGP_ACT_LOGISTIC = 2,
+	NGP_ACT_EXPONENTIAL = 3,
+	NGP_ACT_GELU = 4, /* z * Phi(z), the normal distribution function */
+	NGP_ACT_SILU = 5, /* z * logistic(z) */
+	NGP_ACT_COUNT = 6
+};
+
+/* Activations kept in 8 bits: 32 consecutive features of a row (the last block of a row may be shorter) share a power of
+ * two.  scale = the fp32 exponent field of the block's largest magnitude (at least 109 in NGP_TYPE_F16, whose step 2^-24 is
+ * the type's smallest number); q = rint(v * 2^(133 - scale)), at most 127 in magnitude; a value stands for
+ * q * 2^(scale - 133), which NGP_TYPE_F16 and NGP_TYPE_BF16 hold exactly: off by at most 2^(scale - 134), half a step,
+ * except within half a step of the block's upper end, where it is off by less than one.  A block with a non-finite value
+ * has scale 255 and stands for NaN throughout.  q: [n][q_stride], scale: [n][scale_stride] (one byte per 32 features);
+ * bytes past a row's width (and past its last block's scale) are neither read nor written. */
+typedef struct ngp_checkpoint8 {
+	int8_t* q;
+	uint8_t* scale;
+	uint32_t q_stride;
+	uint32_t scale_stride;
+} ngp_checkpoint8;
+
+/* y = act(x weights^T + bias) + residual, z = x weights^T + bias kept for the backward pass (z in `type`, z8 from fp32). */
+typedef struct ngp_linear_args {
+	uint32_t n;         /* rows (samples) */
+	uint32_t n_in, n_out;
+	int32_t type;       /* NGP_TYPE_F16 or NGP_TYPE_BF16: x, weights, residual, y, z */
+	int32_t activation; /* NGP_ACT_* */
+	uint32_t x_stride, weights_stride, residual_stride, y_stride, z_stride;
+	const void* x;        /* [n][n_in] */
+	const void* weights;  /* [n_out][n_in] */
+	const float* bias;    /* [n_out] or null */
+	const void* residual; /* [n][n_out] or null */
+	void* y;              /* [n][n_out] */
+	void* z;              /* [n][n_out] or null */
+	ngp_checkpoint8 z8;   /* z in 8 bits, or q = scale = null */
+	void* workspace;
+	size_t workspace_bytes;
+} ngp_linear_args;
+ngp_status ngp_linear_workspace(const ngp_linear_args* args, size_t* bytes);
+ngp_status ngp_linear_forward(const ngp_linear_args* args, ngp_stream stream);
+
+/* With p = x if x_activation is NGP_ACT_NONE, else x holds the pre-activation p of the layer below and this layer's input
+ * was act_x(p), rounded to `type`:
+ *   dz = dy act'(z), dx = (dz weights) act_x'(p), dweights = dz^T act_x(p), dbias = the sum of dz over the rows.
+ * dz is rounded to `type` where it enters a product (the matrix cores' operands; dbias sums it in fp32).  The residual's
+ * gradient is dy itself.  dx, dweights and dbias may each be null. */
+typedef struct ngp_linear_backward_args {
+	uint32_t n;
+	uint32_t n_in, n_out;
+	int32_t type;           /* NGP_TYPE_F16 or NGP_TYPE_BF16: dy, z, x, weights, dx */
+	int32_t activation;     /* this layer's: needs z or z8 unless NGP_ACT_NONE */
+	int32_t x_activation;   /* of the layer below */
+	int32_t dweights_type;  /* `type` or NGP_TYPE_F32 */
+	int32_t accumulate;     /* 1: dweights (NGP_TYPE_F32 only) and dbias are added to; 0: overwritten */
+	uint32_t dy_stride, z_stride, x_stride, weights_stride, dx_stride, dweights_stride;
+	const void* dy;       /* [n][n_out] */
+	const void* z;        /* [n][n_out], or null with z8 */
+	ngp_checkpoint8 z8;
+	const void* x;        /* [n][n_in], or null with x8 (neither is needed for dbias alone, or for dx without x_activation) */
+	ngp_checkpoint8 x8;
+	const void* weights;  /* [n_out][n_in] (null without dx) */
+	void* dx;             /* [n][n_in] or null */
+	void* dweights;       /* [n_out][n_in] or null */
+	float* dbias;         /* [n_out] or null */
+	void* workspace;
+	size_t workspace_bytes;
+} ngp_linear_backward_args;
+ngp_status ngp_linear_backward_workspace(const ngp_linear_backward_args* args, size_t* bytes);
+ngp_status ngp_linear_backward(const ngp_linear_backward_args* args, ngp_stream stream);
+
+/* y = (x - mean) rstd gamma + beta per row, rstd = 1 / sqrt(mean((x - mean)^2) + epsilon). */
+typedef struct ngp_layer_norm_args {
+	uint32_t n, width;
+	int32_t type;       /* NGP_TYPE_*: x, y */
+	float epsilon;
+	uint32_t x_stride, y_stride;
+	const void* x;      /* [n][width] */
+	const float* gamma; /* [width] or null (ones) */
+	const float* beta;  /* [width] or null (zeros) */
+	void* y;            /* [n][width] */
+	float* mean;        /* [n] or null: kept for the backward pass */
+	float* rstd;        /* [n] or null */
+	ngp_checkpoint8 y8; /* y in 8 bits (from fp32), or q = scale = null */
+} ngp_layer_norm_args;
+ngp_status ngp_layer_norm_forward(const ngp_layer_norm_args* args, ngp_stream stream);
+
+/* With xh = (x - mean) rstd and g = dy gamma: dx = rstd (g - mean(g) - xh mean(g xh)) + dx_add, dgamma = the sum of dy xh
+ * over the rows, dbeta = the sum of dy. */
+typedef struct ngp_layer_norm_backward_args {
+	uint32_t n, width;
+	int32_t type;         /* NGP_TYPE_*: dy, x, dx_add, dx */
+	int32_t accumulate;   /* 1: dgamma and dbeta are added to; 0: overwritten */
+	uint32_t dy_stride, x_stride, dx_add_stride, dx_stride;
+	const void* dy;       /* [n][width] */
+	const void* x;        /* [n][width], or null with x8 */
+	ngp_checkpoint8 x8;
+	const float* mean;    /* [n], as the forward call wrote them */
+	const float* rstd;    /* [n] */
+	const float* gamma;   /* [width] or null */
+	const void* dx_add;   /* [n][width] or null: the gradient that reaches x by another branch */
+	void* dx;             /* [n][width] or null */
+	float* dgamma;        /* [width] or null */
+	float* dbeta;         /* [width] or null */
+	void* workspace;
+	size_t workspace_bytes;
+} ngp_layer_norm_backward_args;
+ngp_status ngp_layer_norm_backward_workspace(const ngp_layer_norm_backward_args* args, size_t* bytes);
+ngp_status ngp_layer_norm_backward(const ngp_layer_norm_backward_args* args, ngp_stream stream);
+
+/* values [n][width] of `type` (NGP_TYPE_*) -> checkpoint, and the values a checkpoint stands for, rounded to `type`. */
+ngp_status ngp_checkpoint_store(const void* values, uint32_t stride, uint32_t n, uint32_t width, int type,
+                                const ngp_checkpoint8* checkpoint, ngp_stream stream);
+ngp_status ngp_checkpoint_load(const ngp_checkpoint8* checkpoint, uint32_t n, uint32_t width, int type, void* values,
+                               uint32_t stride, ngp_stream stream);
+
 /* --- kernel timers (no reference counterpart: instrumentation for bench.py) ---------- */
 /* When enabled, each hot-path launch group is bracketed by HIP events on the stream it
  * runs on; ngp_timing_read() synchronises those events and returns the summed duration,

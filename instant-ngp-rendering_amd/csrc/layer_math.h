@@ -1,0 +1,112 @@
+// layer_math.h — element types, activations and 8-bit checkpoints of the layer kernels (linear.hip, layer_norm.hip,
+// checkpoint8.hip).  Device code only.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "../../include/ngp_hip.h"
+
+namespace ngp {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+template <class T>
+__device__ __forceinline__ float widen(T v) { return (float)v; }
+template <class T>
+__device__ __forceinline__ T narrow(float v) { return (T)v; }  // to nearest, ties to even
+
+// A value of NGP_ACT_* and its derivative.  exp is the hardware's 2^x (v_exp_f32, ~1 ulp) of x log2(e) rounded once:
+// relative error below 2^-23 (1 + |x|), against the half step 2^-12 / 2^-9 of the 16-bit results.
+__device__ __forceinline__ float act_exp(float x) { return __expf(x); }
+__device__ __forceinline__ float act_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// The normal distribution: Phi(z) and exp(-z^2 / 2).  The lower tail Phi(-a) = exp(-a^2 / 2) R(a), R the scaled
+// complementary error function (half of it), here t P(t) with t = 1 / (1 + 0.31 a) and P the degree-5 polynomial that was
+// fitted to it over 0 <= a <= 14 for the least largest relative error: 4.8e-6.
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+	const float a = fabsf(z);
+	bell = act_exp(-0.5f * z * z);
+	const float t = act_rcp(__builtin_fmaf(0.31f, a, 1.0f));
+	float p = -0.0739346937707959f;
+	p = __builtin_fmaf(p, t, 0.18046493448939863f);
+	p = __builtin_fmaf(p, t, 0.015730865524092818f);
+	p = __builtin_fmaf(p, t, 0.13343541794249958f);
+	p = __builtin_fmaf(p, t, 0.12044041920221424f);
+	p = __builtin_fmaf(p, t, 0.12386071695430309f);
+	const float tail = bell * t * p;
+	return z < 0.0f ? tail : 1.0f - tail;
+}
+
+__device__ __forceinline__ float act_value(int act, float z) {
+	float bell;
+	switch (act) {
+		case NGP_ACT_RELU: return z <= 0.0f ? 0.0f : z;  // a NaN stays one
+		case NGP_ACT_LOGISTIC: return act_rcp(1.0f + act_exp(-z));
+		case NGP_ACT_EXPONENTIAL: return act_exp(z);
+		case NGP_ACT_GELU: return z * normal_cdf(z, bell);
+		case NGP_ACT_SILU: return z * act_rcp(1.0f + act_exp(-z));
+		default: return z;
+	}
+}
+
+__device__ __forceinline__ float act_slope(int act, float z) {
+	switch (act) {
+		case NGP_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+		case NGP_ACT_LOGISTIC: {
+			const float s = act_rcp(1.0f + act_exp(-z));
+			return s * act_rcp(1.0f + act_exp(z));  // 1 - s without the cancellation
+		}
+		case NGP_ACT_EXPONENTIAL: return act_exp(z);
+		case NGP_ACT_GELU: {
+			float bell;
+			const float c = normal_cdf(z, bell);
+			return __builtin_fmaf(z * 0.3989422804014327f, bell, c);
+		}
+		case NGP_ACT_SILU: {
+			const float s = act_rcp(1.0f + act_exp(-z));
+			return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+		}
+		default: return 1.0f;
+	}
+}
+
+// ---- 8-bit checkpoints (ngp_checkpoint8) ----------------------------------------------------------------------
+// A block's scale byte from the largest magnitude's bit pattern (patterns of non-negative floats order as the floats do,
+// infinities and NaNs above all finite ones: their exponent field is 255, which marks the block).
+template <class T>
+__device__ __forceinline__ uint32_t checkpoint_scale(uint32_t max_bits) {
+	const uint32_t e = max_bits >> 23;
+	return std::is_same_v<T, f16> ? (e < 109u ? 109u : e) : e;
+}
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// ldexp keeps the power of two exact over the whole range (133 - scale reaches past the largest float's exponent)
+__device__ __forceinline__ int checkpoint_q(float v, uint32_t scale) {
+	const float q = rintf(ldexpf(v, 133 - (int)scale));
+	return scale == 255u ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+__device__ __forceinline__ float checkpoint_value(int q, uint32_t scale) {
+	return scale == 255u ? __uint_as_float(0x7fc00000u) : ldexpf((float)q, (int)scale - 133);
+}
+
+// Activations as a backward pass finds them: [rows][stride] of T, or a checkpoint (v null), or absent (both null).
+template <class T>
+struct Kept {
+	const T* v = nullptr;
+	size_t stride = 0;
+	const int8_t* q = nullptr;
+	const uint8_t* scale = nullptr;
+	size_t q_stride = 0, scale_stride = 0;
+	__device__ __forceinline__ float at(size_t i, uint32_t j) const {
+		return v ? widen(v[i * stride + j]) : checkpoint_value(q[i * q_stride + j], scale[i * scale_stride + (j >> 5)]);
+	}
+};
+
+template <class T>
+inline Kept<T> kept(const void* v, uint32_t stride, const ngp_checkpoint8& c) {
+	return Kept<T>{static_cast<const T*>(v), stride, c.q, c.scale, c.q_stride, c.scale_stride};
+}
+
+}  // namespace ngp

@@ -27,6 +27,17 @@ void run_error_map_cdf(const float* error_map, uint32_t n_images, uint32_t rx, u
                        float* cdf_y, float* cdf_img, hipStream_t s);
 void run_accumulate_tonemap(const float* frame, float* accum, float* out, uint32_t W, uint32_t H, uint32_t spp,
                             int color_space, float exposure, const float* bg, int output_srgb, hipStream_t s);
+size_t linear_workspace(const ngp_linear_args& a);
+void run_linear_forward(const ngp_linear_args& a, hipStream_t s);
+size_t linear_backward_workspace(const ngp_linear_backward_args& a);
+void run_linear_backward(const ngp_linear_backward_args& a, hipStream_t s);
+void run_layer_norm_forward(const ngp_layer_norm_args& a, hipStream_t s);
+size_t layer_norm_backward_workspace(const ngp_layer_norm_backward_args& a);
+void run_layer_norm_backward(const ngp_layer_norm_backward_args& a, hipStream_t s);
+void run_checkpoint_store(const void* v, uint32_t stride, uint32_t n, uint32_t width, int type, const ngp_checkpoint8& c,
+                          hipStream_t s);
+void run_checkpoint_load(const ngp_checkpoint8& c, uint32_t n, uint32_t width, int type, void* v, uint32_t stride,
+                         hipStream_t s);
 }  // namespace ngp
 
 using namespace ngp;
@@ -782,6 +793,239 @@ ngp_status ngp_timing_read(ngp_model* m, int timer, double* total_ms, uint64_t* 
 			t.units[timer] = 0;
 			t.launches[timer] = 0;
 		}
+	});
+}
+
+// --- layers of any width -----------------------------------------------------------------
+
+// The stream's own device while a model-free call launches on it (the null stream's is the current one).
+namespace {
+struct OnDeviceOf {
+	int before = -1;
+	explicit OnDeviceOf(hipStream_t s) {
+		if (reinterpret_cast<uintptr_t>(s) <= 2) return;  // null, legacy and per-thread streams
+		hipDevice_t dev;
+		int now;
+		NGP_HIP_CHECK(hipStreamGetDevice(s, &dev));
+		NGP_HIP_CHECK(hipGetDevice(&now));
+		if (dev == now) return;
+		NGP_HIP_CHECK(hipSetDevice(dev));
+		before = now;
+	}
+	~OnDeviceOf() {
+		if (before >= 0) (void)hipSetDevice(before);
+	}
+};
+}  // namespace
+
+constexpr uint32_t LAYER_WIDTH_MAX = 65536, LAYER_STRIDE_END = 1u << 22, LAYER_ROWS_MAX = 0x7fffffffu;
+
+static size_t type_size(int type) { return type == NGP_TYPE_F32 ? 4 : 2; }
+static void require_type(int type) {
+	require(type == NGP_TYPE_F32 || type == NGP_TYPE_F16 || type == NGP_TYPE_BF16, "type must be an NGP_TYPE_*");
+}
+static void require_type16(int type) {
+	require(type == NGP_TYPE_F16 || type == NGP_TYPE_BF16, "linear layers take NGP_TYPE_F16 or NGP_TYPE_BF16");
+}
+static void require_act(int act) { require(act >= 0 && act < NGP_ACT_COUNT, "activation must be an NGP_ACT_*"); }
+static void require_width(uint32_t width) {
+	require(width >= 1 && width <= LAYER_WIDTH_MAX, "widths must be in [1, 65536]");
+}
+static void require_rows(uint32_t n) { require(n <= LAYER_ROWS_MAX, "at most 2^31 - 1 rows"); }
+// a matrix that is there: aligned to its elements, a stride that holds its rows
+static void require_matrix(const void* p, uint32_t stride, uint32_t width, size_t element) {
+	if (!p) return;
+	require(reinterpret_cast<uintptr_t>(p) % element == 0, "a matrix must be aligned to its elements");
+	require(stride >= width && stride < LAYER_STRIDE_END, "a stride must be at least the width and below 2^22");
+}
+static void require_checkpoint(const ngp_checkpoint8& c, uint32_t width) {
+	require(!c.q == !c.scale, "a checkpoint has both q and scale, or neither");
+	if (!c.q) return;
+	require(c.q_stride >= width && c.q_stride < LAYER_STRIDE_END, "a checkpoint's q_stride must be at least the width and below 2^22");
+	require(c.scale_stride >= (width + 31) / 32 && c.scale_stride < LAYER_STRIDE_END,
+	        "a checkpoint's scale_stride must hold a byte per 32 features and be below 2^22");
+}
+static void require_f32(const float* p) {
+	require(reinterpret_cast<uintptr_t>(p) % sizeof(float) == 0, "an fp32 vector must be aligned to its elements");
+}
+static void require_workspace(const void* p, size_t bytes, size_t need) {
+	if (!need) return;
+	require(p && bytes >= need, "the workspace is smaller than the matching *_workspace call says");
+	require(reinterpret_cast<uintptr_t>(p) % 16 == 0, "the workspace must be 16-byte aligned");
+}
+
+static void check_linear(const ngp_linear_args* a) {
+	require(a, "null argument");
+	require_type16(a->type);
+	require_act(a->activation);
+	require_rows(a->n);
+	require_width(a->n_in);
+	require_width(a->n_out);
+	require(a->n == 0 || (a->x && a->weights && a->y), "null argument");
+	require_matrix(a->x, a->x_stride, a->n_in, 2);
+	require_matrix(a->weights, a->weights_stride, a->n_in, 2);
+	require_matrix(a->residual, a->residual_stride, a->n_out, 2);
+	require_matrix(a->y, a->y_stride, a->n_out, 2);
+	require_matrix(a->z, a->z_stride, a->n_out, 2);
+	require_f32(a->bias);
+	require_checkpoint(a->z8, a->n_out);
+	require(!a->y || (a->y != a->x && a->y != a->weights && a->y != a->z), "y must not be x, weights or z");
+	require(!a->z || (a->z != a->x && a->z != a->weights && a->z != a->residual), "z must not be an input");
+	require(!a->y || a->y != a->residual || a->y_stride == a->residual_stride, "y in the place of residual needs its stride");
+}
+
+ngp_status ngp_linear_workspace(const ngp_linear_args* a, size_t* bytes) {
+	return guarded([&] {
+		check_linear(a);
+		require(bytes, "null argument");
+		*bytes = linear_workspace(*a);
+	});
+}
+
+ngp_status ngp_linear_forward(const ngp_linear_args* a, ngp_stream s) {
+	return guarded([&] {
+		check_linear(a);
+		require_workspace(a->workspace, a->workspace_bytes, linear_workspace(*a));
+		OnDeviceOf on(S(s));
+		run_linear_forward(*a, S(s));
+	});
+}
+
+static void check_linear_backward(const ngp_linear_backward_args* a) {
+	require(a, "null argument");
+	require_type16(a->type);
+	require_act(a->activation);
+	require_act(a->x_activation);
+	require_rows(a->n);
+	require_width(a->n_in);
+	require_width(a->n_out);
+	require(a->accumulate == 0 || a->accumulate == 1, "accumulate must be 0 or 1");
+	if (a->dweights) {
+		require(a->dweights_type == a->type || a->dweights_type == NGP_TYPE_F32, "dweights_type must be type or NGP_TYPE_F32");
+		require(!a->accumulate || a->dweights_type == NGP_TYPE_F32, "dweights accumulates in NGP_TYPE_F32 only");
+		require_matrix(a->dweights, a->dweights_stride, a->n_in, type_size(a->dweights_type));
+	}
+	require_checkpoint(a->z8, a->n_out);
+	require_checkpoint(a->x8, a->n_in);
+	require(!(a->z && a->z8.q) && !(a->x && a->x8.q), "activations are kept in 16 bits or in 8, not in both");
+	if (a->n) {
+		require(a->dy, "null argument");
+		require(a->activation == NGP_ACT_NONE || a->z || a->z8.q, "an activation's backward pass needs z or z8");
+		require(!a->dweights || a->x || a->x8.q, "dweights needs x or x8");
+		require(!a->dx || a->weights, "dx needs the weights");
+		require(!a->dx || a->x_activation == NGP_ACT_NONE || a->x || a->x8.q, "x_activation needs x or x8");
+	}
+	require_matrix(a->dy, a->dy_stride, a->n_out, 2);
+	require_matrix(a->z, a->z_stride, a->n_out, 2);
+	require_matrix(a->x, a->x_stride, a->n_in, 2);
+	require_matrix(a->weights, a->weights_stride, a->n_in, 2);
+	require_matrix(a->dx, a->dx_stride, a->n_in, 2);
+	require_f32(a->dbias);
+	require(!a->dx || (a->dx != a->dy && a->dx != a->z && a->dx != a->x && a->dx != a->weights && a->dx != a->dweights),
+	        "dx must not be an input or dweights");
+	require(!a->dweights || (a->dweights != a->dy && a->dweights != a->z && a->dweights != a->x && a->dweights != a->weights),
+	        "dweights must not be an input");
+}
+
+ngp_status ngp_linear_backward_workspace(const ngp_linear_backward_args* a, size_t* bytes) {
+	return guarded([&] {
+		check_linear_backward(a);
+		require(bytes, "null argument");
+		*bytes = linear_backward_workspace(*a);
+	});
+}
+
+ngp_status ngp_linear_backward(const ngp_linear_backward_args* a, ngp_stream s) {
+	return guarded([&] {
+		check_linear_backward(a);
+		require_workspace(a->workspace, a->workspace_bytes, linear_backward_workspace(*a));
+		OnDeviceOf on(S(s));
+		run_linear_backward(*a, S(s));
+	});
+}
+
+ngp_status ngp_layer_norm_forward(const ngp_layer_norm_args* a, ngp_stream s) {
+	return guarded([&] {
+		require(a, "null argument");
+		require_type(a->type);
+		require_rows(a->n);
+		require_width(a->width);
+		require(a->n == 0 || (a->x && a->y), "null argument");
+		require(a->epsilon >= 0.0f, "epsilon must not be negative");
+		require_matrix(a->x, a->x_stride, a->width, type_size(a->type));
+		require_matrix(a->y, a->y_stride, a->width, type_size(a->type));
+		require_checkpoint(a->y8, a->width);
+		for (const float* p : {a->gamma, a->beta, (const float*)a->mean, (const float*)a->rstd}) require_f32(p);
+		require(!a->y || a->y != a->x, "y must not be x");
+		OnDeviceOf on(S(s));
+		run_layer_norm_forward(*a, S(s));
+	});
+}
+
+static void check_layer_norm_backward(const ngp_layer_norm_backward_args* a) {
+	require(a, "null argument");
+	require_type(a->type);
+	require_rows(a->n);
+	require_width(a->width);
+	require(a->accumulate == 0 || a->accumulate == 1, "accumulate must be 0 or 1");
+	require_checkpoint(a->x8, a->width);
+	require(!(a->x && a->x8.q), "activations are kept in 16 bits or in 8, not in both");
+	require(a->n == 0 || (a->dy && (a->x || a->x8.q) && a->mean && a->rstd), "null argument");
+	const size_t element = type_size(a->type);
+	require_matrix(a->dy, a->dy_stride, a->width, element);
+	require_matrix(a->x, a->x_stride, a->width, element);
+	require_matrix(a->dx_add, a->dx_add_stride, a->width, element);
+	require_matrix(a->dx, a->dx_stride, a->width, element);
+	for (const float* p : {a->mean, a->rstd, a->gamma, (const float*)a->dgamma, (const float*)a->dbeta}) require_f32(p);
+	require(!a->dx || (a->dx != a->dy && a->dx != a->x), "dx must not be dy or x");
+	require(!a->dx || a->dx != a->dx_add || a->dx_stride == a->dx_add_stride, "dx in the place of dx_add needs its stride");
+	require(!a->dgamma || a->dgamma != a->dbeta, "dgamma must not be dbeta");
+}
+
+ngp_status ngp_layer_norm_backward_workspace(const ngp_layer_norm_backward_args* a, size_t* bytes) {
+	return guarded([&] {
+		check_layer_norm_backward(a);
+		require(bytes, "null argument");
+		*bytes = layer_norm_backward_workspace(*a);
+	});
+}
+
+ngp_status ngp_layer_norm_backward(const ngp_layer_norm_backward_args* a, ngp_stream s) {
+	return guarded([&] {
+		check_layer_norm_backward(a);
+		require_workspace(a->workspace, a->workspace_bytes, layer_norm_backward_workspace(*a));
+		OnDeviceOf on(S(s));
+		run_layer_norm_backward(*a, S(s));
+	});
+}
+
+static void check_checkpoint(const void* values, uint32_t stride, uint32_t n, uint32_t width, int type, const ngp_checkpoint8* c) {
+	require(c, "null argument");
+	require_type(type);
+	require_rows(n);
+	require_width(width);
+	require(n == 0 || (values && c->q && c->scale), "null argument");
+	require_matrix(values, stride, width, type_size(type));
+	require_checkpoint(*c, width);
+}
+
+ngp_status ngp_checkpoint_store(const void* values, uint32_t stride, uint32_t n, uint32_t width, int type,
+                                const ngp_checkpoint8* checkpoint, ngp_stream s) {
+	return guarded([&] {
+		check_checkpoint(values, stride, n, width, type, checkpoint);
+		if (!n) return;
+		OnDeviceOf on(S(s));
+		run_checkpoint_store(values, stride, n, width, type, *checkpoint, S(s));
+	});
+}
+
+ngp_status ngp_checkpoint_load(const ngp_checkpoint8* checkpoint, uint32_t n, uint32_t width, int type, void* values,
+                               uint32_t stride, ngp_stream s) {
+	return guarded([&] {
+		check_checkpoint(values, stride, n, width, type, checkpoint);
+		if (!n) return;
+		OnDeviceOf on(S(s));
+		run_checkpoint_load(*checkpoint, n, width, type, values, stride, S(s));
 	});
 }
 

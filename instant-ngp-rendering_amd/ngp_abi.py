@@ -134,6 +134,52 @@ class Tuning(C.Structure):
     ]
 
 
+class Checkpoint8(C.Structure):
+    """ngp_checkpoint8: activations in 8 bits, 32 consecutive features of a row to a power of two."""
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("q_stride", C.c_uint32), ("scale_stride", C.c_uint32)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_uint32), ("n_in", C.c_uint32), ("n_out", C.c_uint32), ("type", C.c_int32), ("activation", C.c_int32),
+        ("x_stride", C.c_uint32), ("weights_stride", C.c_uint32), ("residual_stride", C.c_uint32),
+        ("y_stride", C.c_uint32), ("z_stride", C.c_uint32),
+        ("x", C.c_void_p), ("weights", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+        ("z", C.c_void_p), ("z8", Checkpoint8), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LinearBackwardArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_uint32), ("n_in", C.c_uint32), ("n_out", C.c_uint32), ("type", C.c_int32), ("activation", C.c_int32),
+        ("x_activation", C.c_int32), ("dweights_type", C.c_int32), ("accumulate", C.c_int32),
+        ("dy_stride", C.c_uint32), ("z_stride", C.c_uint32), ("x_stride", C.c_uint32), ("weights_stride", C.c_uint32),
+        ("dx_stride", C.c_uint32), ("dweights_stride", C.c_uint32),
+        ("dy", C.c_void_p), ("z", C.c_void_p), ("z8", Checkpoint8), ("x", C.c_void_p), ("x8", Checkpoint8),
+        ("weights", C.c_void_p), ("dx", C.c_void_p), ("dweights", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LayerNormArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_uint32), ("width", C.c_uint32), ("type", C.c_int32), ("epsilon", C.c_float),
+        ("x_stride", C.c_uint32), ("y_stride", C.c_uint32),
+        ("x", C.c_void_p), ("gamma", C.c_void_p), ("beta", C.c_void_p), ("y", C.c_void_p), ("mean", C.c_void_p),
+        ("rstd", C.c_void_p), ("y8", Checkpoint8),
+    ]
+
+
+class LayerNormBackwardArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_uint32), ("width", C.c_uint32), ("type", C.c_int32), ("accumulate", C.c_int32),
+        ("dy_stride", C.c_uint32), ("x_stride", C.c_uint32), ("dx_add_stride", C.c_uint32), ("dx_stride", C.c_uint32),
+        ("dy", C.c_void_p), ("x", C.c_void_p), ("x8", Checkpoint8), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+        ("gamma", C.c_void_p), ("dx_add", C.c_void_p), ("dx", C.c_void_p), ("dgamma", C.c_void_p),
+        ("dbeta", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # latent-code rows (include/ngp_hip.h NGP_EXTRA_ROW / NGP_EXTRA_DIMS_MAX)
 EXTRA_ROW = 32
 EXTRA_DIMS_MAX = 32
@@ -145,6 +191,10 @@ SCRATCH_RAY_NUMSTEPS, SCRATCH_COORDS, SCRATCH_MLP_OUT, SCRATCH_RAY_COMPACTED, SC
     SCRATCH_COMPACT_COORDS, SCRATCH_RAY_EVALUATED, SCRATCH_VIOLATIONS = range(9)
 
 RENDER_SHADE, RENDER_AO, RENDER_NORMALS, RENDER_POSITIONS, RENDER_DEPTH, RENDER_COST, RENDER_SLICE = range(7)
+
+# the layers' element types and activations
+TYPE_F32, TYPE_F16, TYPE_BF16 = range(3)
+ACT_NONE, ACT_RELU, ACT_LOGISTIC, ACT_EXPONENTIAL, ACT_GELU, ACT_SILU = range(6)
 
 TIMERS = ["train_sampler", "train_encode", "train_mlp_infer", "train_loss", "train_mlp_bwd", "train_encode_bwd",
           "optimizer", "grid_update", "render_encode", "render_mlp", "render_march"]
@@ -193,6 +243,17 @@ EXPORTS = {
     "ngp_render": (C.c_int, [C.c_void_p, C.POINTER(RenderArgs), C.c_void_p, C.c_void_p, C.c_void_p]),
     "ngp_accumulate_tonemap": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
                                          C.c_int, C.c_float, C.POINTER(C.c_float), C.c_int, C.c_void_p]),
+    "ngp_linear_workspace": (C.c_int, [C.POINTER(LinearArgs), C.POINTER(C.c_size_t)]),
+    "ngp_linear_forward": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p]),
+    "ngp_linear_backward_workspace": (C.c_int, [C.POINTER(LinearBackwardArgs), C.POINTER(C.c_size_t)]),
+    "ngp_linear_backward": (C.c_int, [C.POINTER(LinearBackwardArgs), C.c_void_p]),
+    "ngp_layer_norm_forward": (C.c_int, [C.POINTER(LayerNormArgs), C.c_void_p]),
+    "ngp_layer_norm_backward_workspace": (C.c_int, [C.POINTER(LayerNormBackwardArgs), C.POINTER(C.c_size_t)]),
+    "ngp_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormBackwardArgs), C.c_void_p]),
+    "ngp_checkpoint_store": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.POINTER(Checkpoint8),
+                                       C.c_void_p]),
+    "ngp_checkpoint_load": (C.c_int, [C.POINTER(Checkpoint8), C.c_uint32, C.c_uint32, C.c_int, C.c_void_p, C.c_uint32,
+                                      C.c_void_p]),
     "ngp_timing_enable": (C.c_int, [C.c_void_p, C.c_int]),
     "ngp_timing_read": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_uint64),
                                   C.POINTER(C.c_uint32), C.c_int]),
