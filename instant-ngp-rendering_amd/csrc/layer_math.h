@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
 #include <type_traits>
 
 #include "../../include/ngp_hip.h"
@@ -73,6 +74,57 @@ __device__ __forceinline__ float act_slope(int act, float z) {
 	}
 }
 
+// Eight neighbouring values at once: one branch on the activation, not eight.
+__device__ __forceinline__ void act_values(int act, float (&v)[8]) {
+	switch (act) {
+		case NGP_ACT_RELU: for (float& x : v) x = act_value(NGP_ACT_RELU, x); break;
+		case NGP_ACT_LOGISTIC: for (float& x : v) x = act_value(NGP_ACT_LOGISTIC, x); break;
+		case NGP_ACT_EXPONENTIAL: for (float& x : v) x = act_value(NGP_ACT_EXPONENTIAL, x); break;
+		case NGP_ACT_GELU: for (float& x : v) x = act_value(NGP_ACT_GELU, x); break;
+		case NGP_ACT_SILU: for (float& x : v) x = act_value(NGP_ACT_SILU, x); break;
+		default: break;
+	}
+}
+__device__ __forceinline__ void act_slopes(int act, float (&v)[8]) {
+	switch (act) {
+		case NGP_ACT_RELU: for (float& x : v) x = act_slope(NGP_ACT_RELU, x); break;
+		case NGP_ACT_LOGISTIC: for (float& x : v) x = act_slope(NGP_ACT_LOGISTIC, x); break;
+		case NGP_ACT_EXPONENTIAL: for (float& x : v) x = act_slope(NGP_ACT_EXPONENTIAL, x); break;
+		case NGP_ACT_GELU: for (float& x : v) x = act_slope(NGP_ACT_GELU, x); break;
+		case NGP_ACT_SILU: for (float& x : v) x = act_slope(NGP_ACT_SILU, x); break;
+		default: for (float& x : v) x = 1.0f; break;
+	}
+}
+
+// Eight neighbouring elements of a row that has `left` of them left, at p; one wide access where `wide` says that all
+// rows start on 16 bytes (fp32: two).
+template <class T>
+using v8 = T __attribute__((ext_vector_type(8), aligned(16)));
+template <class T>
+__device__ __forceinline__ void load8(const T* p, uint32_t left, bool wide, float (&v)[8]) {
+	if (wide && left >= 8) {
+		const v8<T> x = *reinterpret_cast<const v8<T>*>(p);
+#pragma unroll
+		for (int k = 0; k < 8; ++k) v[k] = widen(x[k]);
+	} else {
+#pragma unroll
+		for (int k = 0; k < 8; ++k) v[k] = (uint32_t)k < left ? widen(p[k]) : 0.0f;
+	}
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, uint32_t left, bool wide, const float (&v)[8]) {
+	if (wide && left >= 8) {
+		v8<T> x;
+#pragma unroll
+		for (int k = 0; k < 8; ++k) x[k] = narrow<T>(v[k]);
+		*reinterpret_cast<v8<T>*>(p) = x;
+	} else {
+#pragma unroll
+		for (int k = 0; k < 8; ++k)
+			if ((uint32_t)k < left) p[k] = narrow<T>(v[k]);
+	}
+}
+
 // ---- 8-bit checkpoints (ngp_checkpoint8) ----------------------------------------------------------------------
 // A block's scale byte from the largest magnitude's bit pattern (patterns of non-negative floats order as the floats do,
 // infinities and NaNs above all finite ones: their exponent field is 255, which marks the block).
@@ -91,6 +143,30 @@ __device__ __forceinline__ float checkpoint_value(int q, uint32_t scale) {
 	return scale == 255u ? __uint_as_float(0x7fc00000u) : ldexpf((float)q, (int)scale - 133);
 }
 
+// Eight neighbouring values of one block (the first at a multiple of 8) to and from a checkpoint's row.
+__device__ __forceinline__ void checkpoint_store8(int8_t* q, uint32_t left, bool wide, uint32_t scale, const float (&v)[8]) {
+	uint32_t w[2] = {0, 0};
+#pragma unroll
+	for (int k = 0; k < 8; ++k) w[k / 4] |= ((uint32_t)checkpoint_q(v[k], scale) & 0xffu) << (8 * (k % 4));
+	if (wide && left >= 8) {
+		*reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+	} else {
+#pragma unroll
+		for (int k = 0; k < 8; ++k)
+			if ((uint32_t)k < left) q[k] = (int8_t)(w[k / 4] >> (8 * (k % 4)));
+	}
+}
+__device__ __forceinline__ void checkpoint_load8(const int8_t* q, uint32_t left, bool wide, uint32_t scale, float (&v)[8]) {
+	if (wide && left >= 8) {
+		const uint2 w = *reinterpret_cast<const uint2*>(q);
+#pragma unroll
+		for (int k = 0; k < 8; ++k) v[k] = checkpoint_value((int8_t)((k < 4 ? w.x : w.y) >> (8 * (k % 4))), scale);
+	} else {
+#pragma unroll
+		for (int k = 0; k < 8; ++k) v[k] = (uint32_t)k < left ? checkpoint_value(q[k], scale) : 0.0f;
+	}
+}
+
 // Activations as a backward pass finds them: [rows][stride] of T, or a checkpoint (v null), or absent (both null).
 template <class T>
 struct Kept {
@@ -99,14 +175,21 @@ struct Kept {
 	const int8_t* q = nullptr;
 	const uint8_t* scale = nullptr;
 	size_t q_stride = 0, scale_stride = 0;
-	__device__ __forceinline__ float at(size_t i, uint32_t j) const {
-		return v ? widen(v[i * stride + j]) : checkpoint_value(q[i * q_stride + j], scale[i * scale_stride + (j >> 5)]);
+	bool wide = false;  // rows start on 16 bytes (a checkpoint's: on 8)
+	__device__ __forceinline__ void at8(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const {
+		if (v) load8(v + i * stride + j, left, wide, x);
+		else checkpoint_load8(q + i * q_stride + j, left, wide, scale[i * scale_stride + (j >> 5)], x);
 	}
 };
 
+inline bool wide_rows(const void* p, size_t stride, size_t element, size_t bytes = 16) {
+	return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * element % bytes == 0;
+}
+
 template <class T>
 inline Kept<T> kept(const void* v, uint32_t stride, const ngp_checkpoint8& c) {
-	return Kept<T>{static_cast<const T*>(v), stride, c.q, c.scale, c.q_stride, c.scale_stride};
+	return Kept<T>{static_cast<const T*>(v), stride, c.q, c.scale, c.q_stride, c.scale_stride,
+	               v ? wide_rows(v, stride, sizeof(T)) : wide_rows(c.q, c.q_stride, 1, 8)};
 }
 
 }  // namespace ngp

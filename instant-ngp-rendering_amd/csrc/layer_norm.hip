@@ -52,6 +52,11 @@ __global__ void __launch_bounds__(NORM_BLOCK) k_norm_forward(ngp_layer_norm_args
 }
 
 template <class T>
+__device__ __forceinline__ float at(const Kept<T>& x, size_t i, uint32_t j) {
+	return x.v ? widen(x.v[i * x.stride + j]) : checkpoint_value(x.q[i * x.q_stride + j], x.scale[i * x.scale_stride + (j >> 5)]);
+}
+
+template <class T>
 __global__ void __launch_bounds__(NORM_BLOCK) k_norm_backward_rows(ngp_layer_norm_backward_args a) {
 	const size_t i = blockIdx.x;
 	const Kept<T> x = {static_cast<const T*>(a.x), a.x_stride, a.x8.q, a.x8.scale, a.x8.q_stride, a.x8.scale_stride};
@@ -61,13 +66,13 @@ __global__ void __launch_bounds__(NORM_BLOCK) k_norm_backward_rows(ngp_layer_nor
 	for (uint32_t j = threadIdx.x; j < a.width; j += NORM_BLOCK) {
 		const float g = widen(dy[j]) * (a.gamma ? a.gamma[j] : 1.0f);
 		s0 += g;
-		s1 += g * ((x.at(i, j) - mean) * rstd);
+		s1 += g * ((at(x, i, j) - mean) * rstd);
 	}
 	s0 = block_sum(s0) / (float)a.width;
 	s1 = block_sum(s1) / (float)a.width;
 	for (uint32_t j = threadIdx.x; j < a.width; j += NORM_BLOCK) {
 		const float g = widen(dy[j]) * (a.gamma ? a.gamma[j] : 1.0f);
-		float d = rstd * (g - s0 - (x.at(i, j) - mean) * rstd * s1);
+		float d = rstd * (g - s0 - (at(x, i, j) - mean) * rstd * s1);
 		if (a.dx_add) d += widen(static_cast<const T*>(a.dx_add)[i * a.dx_add_stride + j]);
 		static_cast<T*>(a.dx)[i * a.dx_stride + j] = narrow<T>(d);
 	}
@@ -84,7 +89,7 @@ __global__ void __launch_bounds__(NORM_BLOCK) k_norm_backward_columns(ngp_layer_
 	if (j < a.width) {
 		for (size_t i = begin + w; i < end; i += NORM_BLOCK / 64) {
 			const float d = widen(static_cast<const T*>(a.dy)[i * a.dy_stride + j]);
-			g += d * ((x.at(i, j) - a.mean[i]) * a.rstd[i]);
+			g += d * ((at(x, i, j) - a.mean[i]) * a.rstd[i]);
 			b += d;
 		}
 	}

@@ -2,28 +2,55 @@
 //
 //   forward   z = x W^T + b, y = act(z) + r
 //   backward  dz = dy act'(z), dx = (dz W) act_x'(p), dW = dz^T act_x(p), db = sum of dz
+//
+// Three products C[m][n] = sum over k of P[m][k] Q[n][k], one kernel (k_product):
+//   y:  P = x  [row][k],  Q = W  [row][k]
+//   dx: P = dz [row][k],  Q = W  [k][row]  (k runs over the outputs)
+//   dW: P = dz [k][row],  Q = x  [k][row]  (k runs over the samples)
+#include <algorithm>
+
 #include "layer_math.h"
 #include "ngp_internal.h"
 
 namespace ngp {
 
-// What a product C[m][n] does with its fp32 sums.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+__device__ __forceinline__ f32x16 mfma(f16, s16x8 a, s16x8 b, f32x16 c) {
+	return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8<f16>, a), __builtin_bit_cast(v8<f16>, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(bf16, s16x8 a, s16x8 b, f32x16 c) {
+	return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8<bf16>, a), __builtin_bit_cast(v8<bf16>, b), c, 0, 0, 0);
+}
+
+// ---- what a product does with its fp32 sums, eight neighbouring columns of a row at a time --------------------------
 template <class T>
 struct ForwardOut {
 	const float* bias;
-	int act;
 	const T* residual;
 	T* y;
 	T* z;
 	ngp_checkpoint8 z8;
 	size_t residual_stride, y_stride, z_stride;
-	__device__ __forceinline__ float finish(size_t i, uint32_t j, float z_) const {
-		const float v = z_ + (bias ? bias[j] : 0.0f);
-		if (z) z[i * z_stride + j] = narrow<T>(v);
-		float r = act_value(act, v);
-		if (residual) r += widen(residual[i * residual_stride + j]);
-		y[i * y_stride + j] = narrow<T>(r);
-		return v;
+	int act;
+	bool residual_wide, y_wide, z_wide, z8_wide;
+	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, float (&v)[8], float (&kept)[8]) const {
+#pragma unroll
+		for (int k = 0; k < 8; ++k) v[k] += bias && (uint32_t)k < left ? bias[j + k] : 0.0f;
+#pragma unroll
+		for (int k = 0; k < 8; ++k) kept[k] = v[k];
+		if (z) store8(z + i * z_stride + j, left, z_wide, v);
+		act_values(act, v);
+		if (residual) {
+			float r[8];
+			load8(residual + i * residual_stride + j, left, residual_wide, r);
+#pragma unroll
+			for (int k = 0; k < 8; ++k) v[k] += r[k];
+		}
+		store8(y + i * y_stride + j, left, y_wide, v);
 	}
 };
 
@@ -33,11 +60,18 @@ struct GradientOut {  // dx
 	size_t stride;
 	Kept<T> p;
 	int act;
-	ngp_checkpoint8 z8;  // unused (null)
-	__device__ __forceinline__ float finish(size_t i, uint32_t j, float v) const {
-		if (act != NGP_ACT_NONE) v *= act_slope(act, p.at(i, j));
-		dx[i * stride + j] = narrow<T>(v);
-		return v;
+	bool wide;
+	static constexpr ngp_checkpoint8 z8 = {};
+	static constexpr bool z8_wide = false;
+	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, float (&v)[8], float (&)[8]) const {
+		if (act != NGP_ACT_NONE) {
+			float s[8];
+			p.at8(i, j, left, s);
+			act_slopes(act, s);
+#pragma unroll
+			for (int k = 0; k < 8; ++k) v[k] *= s[k];
+		}
+		store8(dx + i * stride + j, left, wide, v);
 	}
 };
 
@@ -45,177 +79,491 @@ template <class T>
 struct WeightsOut {  // dW
 	void* dw;
 	size_t stride;
-	int f32, accumulate;
-	ngp_checkpoint8 z8;  // unused (null)
-	__device__ __forceinline__ float finish(size_t i, uint32_t j, float v) const {
+	bool f32, accumulate, wide;
+	static constexpr ngp_checkpoint8 z8 = {};
+	static constexpr bool z8_wide = false;
+	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, float (&v)[8], float (&)[8]) const {
 		if (f32) {
 			float* d = static_cast<float*>(dw) + i * stride + j;
-			*d = accumulate ? *d + v : v;
+			if (accumulate) {
+				float o[8];
+				load8(d, left, wide, o);
+#pragma unroll
+				for (int k = 0; k < 8; ++k) v[k] += o[k];
+			}
+			store8(d, left, wide, v);
 		} else {
-			static_cast<T*>(dw)[i * stride + j] = narrow<T>(v);
+			store8(static_cast<T*>(dw) + i * stride + j, left, wide, v);
 		}
-		return v;
 	}
 };
 
-// A product's operand, element by element: kept activations, an activation of them, rounded to T.
-template <class T>
-struct Operand {
-	Kept<T> v;
-	int act = NGP_ACT_NONE;
-	bool by_k = false;  // [k][row] in memory
-	__device__ __forceinline__ float at(size_t row, size_t k) const {
-		const float x = by_k ? v.at(k, (uint32_t)row) : v.at(row, (uint32_t)k);
-		return act == NGP_ACT_NONE ? x : widen(narrow<T>(act_value(act, x)));
+// ---- the product ------------------------------------------------------------------------------------------------------
+// An operand whose rows start on 16 bytes and are multiples of 8 elements long.
+struct Matrix {
+	const void* v;
+	size_t stride;
+};
+
+struct ProductArgs {
+	Matrix p, q;
+	size_t M, K, k_each;  // k_each: how much of K a split takes, a multiple of PRODUCT_K
+	uint32_t N, tiles_m, tiles_n, splits;
+	float* partial;       // [splits][M][N up to 8] where splits > 1
+};
+
+constexpr int PRODUCT_K = 64;   // of K per stage
+constexpr int PRODUCT_THREADS = 256;
+
+// One stage of an operand in LDS: ROWS x 64 elements of 16 bits.  Each wave's load puts 64 chunks of 16 bytes one after
+// another (buffer_load ... lds takes no other order), so rows are spread over the banks by what each lane fetches:
+//  * [row][k] in memory: 128 bytes per row, chunk c of row r holds k chunk c ^ (r & 7); ds_read_b128 of 32 rows' same
+//    k chunk touches every bank equally.
+//  * [k][row] in memory: 2 ROWS bytes per k, chunk c of line k holds rows' chunk c ^ twist(k); ds_read_b64_tr_b16 reads
+//    four k lines x 64 bytes per half wave, which the twist puts on different banks.
+template <class T, int ROWS, bool BY_K>
+struct Stage {
+	static constexpr int BYTES = ROWS * PRODUCT_K * 2;
+	static constexpr int LOADS = BYTES / 16 / PRODUCT_THREADS;
+	static constexpr int LINE = BY_K ? ROWS * 2 : PRODUCT_K * 2;  // bytes
+	static constexpr uint32_t OUTSIDE = 0xfffffff0u;              // past every buffer: the load gives zeros
+	__device__ static __forceinline__ uint32_t twist(uint32_t k) {
+		return LINE >= 256 ? ((k & 3u) << 2) | (k & 2u) : (((k >> 1) & 1u) << 2) | ((k & 1u) << 1);
+	}
+
+	const char* base;       // of the stage's first element (uniform)
+	size_t step;            // bytes to the next stage
+	uint32_t offset[LOADS]; // a thread's chunks
+	uint32_t k_of[LOADS];   // their first k in the stage
+
+	// rows [row0, rows) of the matrix from k0 on
+	__device__ __forceinline__ void begin(const Matrix& m, size_t row0, size_t rows, size_t k0) {
+		const uint32_t left = (uint32_t)min(rows - row0, (size_t)ROWS);
+		base = static_cast<const char*>(m.v) + (BY_K ? k0 * m.stride + row0 : row0 * m.stride + k0) * 2;
+		step = BY_K ? m.stride * (PRODUCT_K * 2) : PRODUCT_K * 2;
+#pragma unroll
+		for (int l = 0; l < LOADS; ++l) {
+			const uint32_t c = threadIdx.x + l * PRODUCT_THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
+			const uint32_t row = BY_K ? (at ^ twist(line)) * 8u : line;
+			k_of[l] = BY_K ? line : (at ^ (line & 7u)) * 8u;
+			offset[l] = row < left ? (BY_K ? k_of[l] * (uint32_t)m.stride + row : row * (uint32_t)m.stride + k_of[l]) * 2u : OUTSIDE;
+		}
+	}
+	// k_left: how much of K is left from this stage on
+	__device__ __forceinline__ void load(char* lds, uint32_t k_left) {
+		const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, 0x7fffffff, 0x00027000);
+		char* wave = lds + (threadIdx.x & ~63u) * 16u;
+#pragma unroll
+		for (int l = 0; l < LOADS; ++l) {
+			const uint32_t at = k_of[l] < k_left ? offset[l] : OUTSIDE;
+			__builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(wave + l * PRODUCT_THREADS * 16), 16, at, 0, 0, 0);
+		}
+		base += step;
 	}
 };
 
-constexpr int TILE = 64, TILE_K = 16;
-
-// C[m][n] = sum over k of P[m][k] Q[n][k]: 64 x 64 per workgroup, 4 x 4 per thread, operands through LDS in fp32.
-template <class T, class Out>
-__global__ void __launch_bounds__(256) k_product(Operand<T> P, Operand<T> Q, size_t M, uint32_t N, size_t K, Out out) {
-	__shared__ float sp[TILE_K][TILE + 1], sq[TILE_K][TILE + 1], sz[TILE][TILE + 1];
-	const size_t m0 = (size_t)blockIdx.x * TILE;
-	const uint32_t n0 = blockIdx.y * TILE;
-	const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-	float c[4][4] = {};
-	for (size_t k0 = 0; k0 < K; k0 += TILE_K) {
-		for (int t = threadIdx.x; t < TILE * TILE_K; t += 256) {
-			// neighbouring threads along whichever index is contiguous in memory
-			const int pr = P.by_k ? t % TILE : t / TILE_K, pk = P.by_k ? t / TILE : t % TILE_K;
-			const int qr = Q.by_k ? t % TILE : t / TILE_K, qk = Q.by_k ? t / TILE : t % TILE_K;
-			sp[pk][pr] = m0 + pr < M && k0 + pk < K ? P.at(m0 + pr, k0 + pk) : 0.0f;
-			sq[qk][qr] = n0 + qr < N && k0 + qk < K ? Q.at(n0 + qr, k0 + qk) : 0.0f;
+// A wave's 32 x 16 fragments of a stage: lane l holds row l % 32 and k = 8 (l / 32) .. + 7 of each 16.
+template <class T, int ROWS, bool BY_K, int TILES>
+struct Fragments {
+	uint32_t offset[BY_K ? TILES : 4];
+	__device__ __forceinline__ void begin(uint32_t row0) {
+		const uint32_t lane = threadIdx.x & 63u;
+		if constexpr (BY_K) {
+			// 16 lanes read 4 k lines x 16 rows and get them transposed: lane j of them row j's four k
+			const uint32_t g = lane >> 4, q = (lane & 15u) >> 2, p = lane & 3u;
+#pragma unroll
+			for (int t = 0; t < TILES; ++t) {
+				const uint32_t chunk = (row0 + t * 32u + 16u * (g & 1u)) / 8u + (p >> 1);
+				offset[t] = (8u * (g >> 1) + q) * (ROWS * 2) + ((chunk ^ Stage<T, ROWS, BY_K>::twist(q)) << 4) + (p & 1u) * 8u;
+			}
+		} else {
+#pragma unroll
+			for (int s = 0; s < 4; ++s)
+				offset[s] = (row0 + (lane & 31u)) * (PRODUCT_K * 2) + (((s * 2u + (lane >> 5)) ^ (lane & 7u)) << 4);
 		}
-		__syncthreads();
-		for (int k = 0; k < TILE_K; ++k)
-			for (int a = 0; a < 4; ++a)
-				for (int b = 0; b < 4; ++b) c[a][b] = __builtin_fmaf(sp[k][tm * 4 + a], sq[k][tn * 4 + b], c[a][b]);
-		__syncthreads();
 	}
-	for (int a = 0; a < 4; ++a)
-		for (int b = 0; b < 4; ++b) {
-			const size_t i = m0 + tm * 4 + a;
-			const uint32_t j = n0 + tn * 4 + b;
-			sz[tm * 4 + a][tn * 4 + b] = i < M && j < N ? out.finish(i, j, c[a][b]) : 0.0f;
+	__device__ __forceinline__ s16x8 read(const char* lds, int s, int t) const {  // the s-th 16 of k, the t-th 32 rows
+		if constexpr (BY_K) {
+			typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+			const char* at = lds + offset[t] + s * 16 * (ROWS * 2);
+			const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+			const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 4 * (ROWS * 2)));
+			return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+		} else {
+			return *reinterpret_cast<const s16x8*>(lds + offset[s] + t * 32 * (PRODUCT_K * 2));
 		}
-	if (!out.z8.q) return;
-	__syncthreads();
-	if (threadIdx.x >= TILE * 2) return;
-	const size_t i = m0 + threadIdx.x / 2;
-	const uint32_t h = threadIdx.x % 2 * 32, j0 = n0 + h;
-	if (i >= M || j0 >= N) return;
-	const float* row = sz[threadIdx.x / 2] + h;
-	uint32_t top = 0;
-	for (int j = 0; j < 32; ++j) top = max(top, magnitude_bits(row[j]));
-	const uint32_t scale = checkpoint_scale<T>(top);
-	for (uint32_t j = 0; j < 32 && j0 + j < N; ++j) out.z8.q[i * out.z8.q_stride + j0 + j] = (int8_t)checkpoint_q(row[j], scale);
-	out.z8.scale[i * out.z8.scale_stride + j0 / 32] = (uint8_t)scale;
+	}
+};
+
+// BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through two LDS buffers: while the matrix cores
+// work on one stage, the next is on its way from memory into the other buffer without passing registers.  P's rows are
+// the matrix instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN>
+__global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) k_product(ProductArgs a, Out out) {
+	constexpr int TM = BM / 64, TN = BN / 64;  // 32 x 32 tiles per wave
+	typedef Stage<T, BM, P_BY_K> PStage;
+	typedef Stage<T, BN, Q_BY_K> QStage;
+	constexpr int STAGE = PStage::BYTES + QStage::BYTES;
+	extern __shared__ __attribute__((aligned(16))) char lds[];
+
+	// workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight tile rows deep, so that
+	// its L2 holds what they share
+	const uint32_t tiles = a.tiles_m * a.tiles_n, all = gridDim.x, xcd = blockIdx.x % 8u;
+	const uint32_t id = xcd * (all / 8u) + min(xcd, all % 8u) + blockIdx.x / 8u;
+	const uint32_t split = id / tiles, tile = id % tiles;
+	const uint32_t group = tile / (8u * a.tiles_n), first = group * 8u, deep = min(8u, a.tiles_m - first);
+	const uint32_t in_group = tile - group * 8u * a.tiles_n;
+	const size_t m0 = (size_t)(first + in_group % deep) * BM;
+	const uint32_t n0 = in_group / deep * BN;
+
+	const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u;
+	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
+	const size_t k0 = split * a.k_each, k1 = min(k0 + a.k_each, a.K);
+	const uint32_t stages = (uint32_t)((k1 - k0 + PRODUCT_K - 1) / PRODUCT_K);
+
+	PStage ps;
+	QStage qs;
+	Fragments<T, BM, P_BY_K, TM> pf;
+	Fragments<T, BN, Q_BY_K, TN> qf;
+	pf.begin(wm);
+	qf.begin(wn);
+	f32x16 c[TN][TM] = {};
+	if (stages) {
+		ps.begin(a.p, m0, a.M, k0);
+		qs.begin(a.q, n0, a.N, k0);
+		auto load = [&](uint32_t s) {
+			const uint32_t left = (uint32_t)min(k1 - k0 - (size_t)s * PRODUCT_K, (size_t)PRODUCT_K);
+			char* to = lds + (s & 1u) * STAGE;
+			ps.load(to, left);
+			qs.load(to + PStage::BYTES, left);
+		};
+		s16x8 p[2][TM], q[2][TN];
+		auto read = [&](const char* from, int s) {
+#pragma unroll
+			for (int t = 0; t < TN; ++t) q[s & 1][t] = qf.read(from + PStage::BYTES, s, t);
+#pragma unroll
+			for (int t = 0; t < TM; ++t) p[s & 1][t] = pf.read(from, s, t);
+		};
+		auto arrived = [] {  // this wave's reads of the one buffer are done and its loads into the other there; then everybody's
+			__builtin_amdgcn_s_waitcnt(0);
+			__syncthreads();
+		};
+		load(0);
+		arrived();
+		if (stages > 1) load(1);
+		read(lds, 0);
+		for (uint32_t s = 0; s < stages; ++s) {
+			const char* now = lds + (s & 1u) * STAGE;
+#pragma unroll
+			for (int k = 0; k < 4; ++k) {
+				if (k < 3) {
+					read(now, k + 1);
+				} else if (s + 1 < stages) {
+					arrived();
+					if (s + 2 < stages) load(s + 2);
+					read(lds + ((s + 1) & 1u) * STAGE, 0);
+				}
+#pragma unroll
+				for (int n = 0; n < TN; ++n)
+#pragma unroll
+					for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k & 1][n], p[k & 1][m], c[n][m]);
+			}
+		}
+	}
+
+	// register r of a 32 x 32 tile: column r % 4 + 8 (r / 4) + 4 (lane / 32), row lane % 32; two groups of four columns
+	// change places between the half waves, which leaves every lane eight neighbouring ones, twice
+	const uint32_t n8 = (a.N + 7u) & ~7u;
+#pragma unroll
+	for (int m = 0; m < TM; ++m) {
+		const size_t i = m0 + wm + m * 32u + (lane & 31u);
+#pragma unroll
+		for (int n = 0; n < TN; ++n) {
+			float v[2][8];
+#pragma unroll
+			for (int h = 0; h < 2; ++h)
+#pragma unroll
+				for (int k = 0; k < 4; ++k) {
+					const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[n][m][8 * h + k]), __float_as_uint(c[n][m][8 * h + 4 + k]),
+					                                                false, false);
+					v[h][k] = __uint_as_float(s[0]);
+					v[h][k + 4] = __uint_as_float(s[1]);
+				}
+			const uint32_t j = n0 + wn + n * 32u + 8u * (lane >> 5);
+			if (a.splits > 1) {
+#pragma unroll
+				for (int h = 0; h < 2; ++h)
+					if (i < a.M && j + 16u * h < n8) store8(a.partial + ((size_t)split * a.M + i) * n8 + j + 16u * h, 8, true, v[h]);
+				continue;
+			}
+			float z[2][8] = {};
+			uint32_t left[2], top = 0;
+#pragma unroll
+			for (int h = 0; h < 2; ++h) {
+				left[h] = i < a.M && j + 16u * h < a.N ? a.N - j - 16u * h : 0u;
+				if (left[h]) out.finish(i, j + 16u * h, left[h], v[h], z[h]);
+#pragma unroll
+				for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left[h] ? magnitude_bits(z[h][k]) : 0u);
+			}
+			if (!out.z8.q) continue;
+			const auto s = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+			const uint32_t scale = checkpoint_scale<T>(max(s[0], s[1]));
+#pragma unroll
+			for (int h = 0; h < 2; ++h)
+				if (left[h]) checkpoint_store8(out.z8.q + i * out.z8.q_stride + j + 16u * h, left[h], out.z8_wide, scale, z[h]);
+			if (left[0] && lane < 32u) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
+		}
+	}
 }
 
-// dz = dy act'(z) and its sums over a share of the rows: 64 columns x rows_each rows per workgroup.
+// The splits' sums, in their order, to where the product would have put them.
+template <class T, class Out>
+__global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ partial, uint32_t splits, size_t M, uint32_t N, Out out) {
+	const uint32_t n8 = (N + 7u) & ~7u, chunks = (N + 31u) / 32u * 4u;  // four threads to a block of 32
+	const size_t t = (size_t)blockIdx.x * 256u + threadIdx.x, i = t / chunks;
+	const uint32_t j = (uint32_t)(t % chunks) * 8u;
+	const bool in = i < M && j < N;
+	float v[8] = {}, z[8] = {};
+	if (in)
+		for (uint32_t s = 0; s < splits; ++s) {
+			float x[8];
+			load8(partial + ((size_t)s * M + i) * n8 + j, 8, true, x);
+#pragma unroll
+			for (int k = 0; k < 8; ++k) v[k] += x[k];
+		}
+	const uint32_t left = in ? N - j : 0u;
+	if (left) out.finish(i, j, left, v, z);
+	if (!out.z8.q) return;
+	uint32_t top = 0;
+#pragma unroll
+	for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left ? magnitude_bits(z[k]) : 0u);
+	top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+	top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+	if (!left) return;
+	const uint32_t scale = checkpoint_scale<T>(top);
+	checkpoint_store8(out.z8.q + i * out.z8.q_stride + j, left, out.z8_wide, scale, z);
+	if (j % 32u == 0) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
+}
+
+// ---- operands that do not lie as the product wants them ---------------------------------------------------------------
+// act(v), rounded to T, in rows of `width` up to 8, filled up with zeros.
 template <class T>
-__global__ void __launch_bounds__(256) k_linear_dz(const T* __restrict__ dy, size_t dy_stride, Kept<T> z, int act, uint32_t n,
-                                                   uint32_t width, uint32_t rows_each, T* dz, float* part) {
-	const uint32_t j = blockIdx.x * 64u + (threadIdx.x & 63u), w = threadIdx.x >> 6;
-	const size_t begin = (size_t)blockIdx.y * rows_each, end = min(begin + rows_each, (size_t)n);
+__global__ void __launch_bounds__(256) k_lay_out(Kept<T> v, int act, size_t rows, uint32_t width, T* __restrict__ to) {
+	const uint32_t chunks = (width + 7u) / 8u;
+	for (size_t t = (size_t)blockIdx.x * 256u + threadIdx.x; t < rows * chunks; t += (size_t)gridDim.x * 256u) {
+		const size_t i = t / chunks;
+		const uint32_t j = (uint32_t)(t % chunks) * 8u;
+		float x[8];
+		v.at8(i, j, width - j, x);
+		act_values(act, x);
+#pragma unroll
+		for (int k = 0; k < 8; ++k) x[k] = j + k < width ? x[k] : 0.0f;
+		store8(to + t * 8u, 8, true, x);
+	}
+}
+
+// dz = dy act'(z), in rows of `width` up to 8 (dz null: not kept), and its sums over a share of the rows.  A workgroup
+// takes 8 * groups columns (groups a power of two up to 32) and 256 / groups rows at a time.
+template <class T>
+__global__ void __launch_bounds__(256) k_linear_dz(Kept<T> dy, Kept<T> z, int act, size_t n, uint32_t width, uint32_t groups,
+                                                   size_t rows_each, T* __restrict__ dz, float* __restrict__ part) {
+	const uint32_t g = threadIdx.x % groups, lines = 256u / groups, j = (blockIdx.x * groups + g) * 8u;
+	const size_t begin = blockIdx.y * rows_each, end = min(begin + rows_each, n);
+	const uint32_t w8 = (width + 7u) & ~7u;
+	float sum[8] = {};
+	if (j < width)
+		for (size_t i = begin + threadIdx.x / groups; i < end; i += lines) {
+			float d[8];
+			dy.at8(i, j, width - j, d);
+			if (act != NGP_ACT_NONE) {
+				float s[8];
+				z.at8(i, j, width - j, s);
+				act_slopes(act, s);
+#pragma unroll
+				for (int k = 0; k < 8; ++k) d[k] = j + k < width ? d[k] * s[k] : 0.0f;
+			}
+			if (dz) store8(dz + i * w8 + j, 8, true, d);
+#pragma unroll
+			for (int k = 0; k < 8; ++k) sum[k] += d[k];
+		}
+	if (!part) return;
+	__shared__ float s[256][9];
+#pragma unroll
+	for (int k = 0; k < 8; ++k) s[threadIdx.x][k] = sum[k];
+	__syncthreads();
+	if (threadIdx.x >= groups * 8u) return;
+	const uint32_t column = blockIdx.x * groups * 8u + threadIdx.x;
+	if (column >= width) return;
+	float total = 0.0f;
+	for (uint32_t l = 0; l < lines; ++l) total += s[l * groups + threadIdx.x / 8u][threadIdx.x % 8u];
+	part[(size_t)blockIdx.y * width + column] = total;
+}
+
+__global__ void __launch_bounds__(256) k_column_sum(const float* __restrict__ part, uint32_t shares, uint32_t width, float* out,
+                                                    int accumulate) {
+	const uint32_t c = threadIdx.x % 16u, line = threadIdx.x / 16u, j = blockIdx.x * 16u + c;
 	float sum = 0.0f;
 	if (j < width)
-		for (size_t i = begin + w; i < end; i += 4) {
-			float d = widen(dy[i * dy_stride + j]);
-			if (act != NGP_ACT_NONE) d *= act_slope(act, z.at(i, j));
-			if (dz) dz[i * width + j] = narrow<T>(d);
-			sum += d;
-		}
-	__shared__ float s[256];
-	s[threadIdx.x] = sum;
+		for (uint32_t k = line; k < shares; k += 16u) sum += part[(size_t)k * width + j];
+	__shared__ float s[16][17];
+	s[line][c] = sum;
 	__syncthreads();
-	const uint32_t t = threadIdx.x;
-	if (part && w == 0 && j < width) part[(size_t)blockIdx.y * width + j] = (s[t] + s[t + 64]) + (s[t + 128] + s[t + 192]);
+	if (line || j >= width) return;
+	for (int l = 1; l < 16; ++l) sum += s[l][c];
+	out[j] = accumulate ? out[j] + sum : sum;
 }
 
-__global__ void k_column_sum(const float* __restrict__ part, uint32_t shares, uint32_t width, float* out, int accumulate) {
-	const uint32_t j = blockIdx.x * 256u + threadIdx.x;
-	if (j >= width) return;
-	float s = 0.0f;
-	for (uint32_t k = 0; k < shares; ++k) s += part[(size_t)k * width + j];
-	out[j] = accumulate ? out[j] + s : s;
-}
-
-size_t linear_workspace(const ngp_linear_args&) { return 0; }
-
+// ---- host ---------------------------------------------------------------------------------------------------------------
 static size_t up16(size_t b) { return (b + 15) & ~(size_t)15; }
-static uint32_t row_shares(uint32_t n) { return std::max(1u, std::min(256u, n / 64u)); }
+static uint32_t up8(uint32_t w) { return (w + 7u) & ~7u; }
 
-struct LinearBackwardPlan {
-	size_t dz = 0, part = 0, bytes = 0;  // offsets in the workspace
+// The workspace as a call deals it out; without `run` nothing is launched and only the size is counted.
+struct Room {
+	char* at;
+	bool run;
+	size_t bytes = 0;
+	template <class U>
+	U* take(size_t count) {
+		U* p = reinterpret_cast<U*>(at + bytes);
+		bytes += up16(count * sizeof(U));
+		return p;
+	}
 };
 
-static LinearBackwardPlan plan(const ngp_linear_backward_args& a) {
-	LinearBackwardPlan p;
-	if (a.activation != NGP_ACT_NONE) p.bytes += up16((size_t)a.n * a.n_out * 2);
-	p.part = p.bytes;
-	if (a.dbias) p.bytes += up16((size_t)row_shares(a.n) * a.n_out * 4);
+struct ProductPlan {
+	int tile = 64;
+	uint32_t tiles_m = 0, tiles_n = 0, splits = 1;
+	size_t k_each = 0;
+};
+
+// The tile: the largest that still gives most of the 256 CUs something to do (a 256 x 256 tile moves a quarter of the bytes
+// of a 64 x 64 one through LDS per multiplication).  K is split where the tiles are too few: until there are about two
+// workgroups per CU, or four stages each.
+static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
+	ProductPlan p;
+	auto tiles = [&](size_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+	p.tile = M > 128 && N > 128 && tiles(256) >= 192 ? 256 : (M > 64 && N > 64 && tiles(128) * (K / 512 + 1) >= 256 ? 128 : 64);
+	p.tiles_m = (uint32_t)((M + p.tile - 1) / p.tile);
+	p.tiles_n = (uint32_t)((N + p.tile - 1) / p.tile);
+	const size_t stages = (K + PRODUCT_K - 1) / PRODUCT_K, count = (size_t)p.tiles_m * p.tiles_n;
+	const size_t splits = count >= 256 ? 1 : std::max<size_t>(1, std::min<size_t>(std::min<size_t>(512 / count, stages / 4), 256));
+	const size_t each = std::max<size_t>(1, (stages + splits - 1) / splits);
+	p.k_each = each * PRODUCT_K;
+	p.splits = stages ? (uint32_t)((stages + each - 1) / each) : 1u;
 	return p;
 }
 
-size_t linear_backward_workspace(const ngp_linear_backward_args& a) { return plan(a).bytes; }
-
-template <class T>
-static void linear_forward(const ngp_linear_args& a, hipStream_t s) {
-	if (!a.n) return;
-	const Operand<T> x{Kept<T>{static_cast<const T*>(a.x), a.x_stride}}, w{Kept<T>{static_cast<const T*>(a.weights), a.weights_stride}};
-	const ForwardOut<T> out{a.bias, a.activation, static_cast<const T*>(a.residual), static_cast<T*>(a.y), static_cast<T*>(a.z),
-	                        a.z8, a.residual_stride, a.y_stride, a.z_stride};
-	k_product<T><<<dim3((a.n + TILE - 1) / TILE, (a.n_out + TILE - 1) / TILE), 256, 0, s>>>(x, w, a.n, a.n_out, a.n_in, out);
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int TILE>
+static void launch_product(const ProductArgs& a, const Out& out, hipStream_t s) {
+	constexpr uint32_t lds = 2 * 2 * TILE * PRODUCT_K * 2;
+	auto kernel = k_product<T, Out, P_BY_K, Q_BY_K, TILE, TILE>;
+	if (lds > 65536)
+		NGP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+	kernel<<<a.tiles_m * a.tiles_n * a.splits, PRODUCT_THREADS, lds, s>>>(a, out);
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
-template <class T>
-static void linear_backward(const ngp_linear_backward_args& a, hipStream_t s) {
-	const LinearBackwardPlan p = plan(a);
-	char* ws = static_cast<char*>(a.workspace);
-	const bool own = a.activation != NGP_ACT_NONE;
-	T* dz_ws = reinterpret_cast<T*>(ws + p.dz);
-	Operand<T> dz{own ? Kept<T>{dz_ws, a.n_out} : Kept<T>{static_cast<const T*>(a.dy), a.dy_stride}};
-	if (own || a.dbias) {
-		const uint32_t shares = row_shares(a.n), each = (a.n + shares - 1) / shares;
-		float* part = a.dbias ? reinterpret_cast<float*>(ws + p.part) : nullptr;
-		k_linear_dz<T><<<dim3((a.n_out + 63) / 64, shares), 256, 0, s>>>(
-		    static_cast<const T*>(a.dy), a.dy_stride, kept<T>(a.z, a.z_stride, a.z8), a.activation, a.n, a.n_out, each,
-		    own ? dz_ws : nullptr, part);
+// C[M][N] = P Q^T to `out`; a Room that does not run only counts what it takes.
+template <class T, class Out, bool P_BY_K, bool Q_BY_K>
+static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size_t K, const Out& out, Room& room, hipStream_t s) {
+	if (!M) return;
+	const ProductPlan plan = plan_product(M, N, K);
+	ProductArgs a{p, q, M, K, plan.k_each, N, plan.tiles_m, plan.tiles_n, plan.splits, nullptr};
+	if (plan.splits > 1) a.partial = room.take<float>((size_t)plan.splits * M * up8(N));
+	if (!room.run) return;
+	if (plan.tile == 256) launch_product<T, Out, P_BY_K, Q_BY_K, 256>(a, out, s);
+	else if (plan.tile == 128) launch_product<T, Out, P_BY_K, Q_BY_K, 128>(a, out, s);
+	else launch_product<T, Out, P_BY_K, Q_BY_K, 64>(a, out, s);
+	if (plan.splits > 1) {
+		const size_t items = M * ((N + 31u) / 32u * 4u);
+		k_product_join<T, Out><<<(uint32_t)((items + 255) / 256), 256, 0, s>>>(a.partial, plan.splits, M, N, out);
 		NGP_HIP_CHECK(hipGetLastError());
-		if (a.dbias) {
-			k_column_sum<<<(a.n_out + 255) / 256, 256, 0, s>>>(part, shares, a.n_out, a.dbias, a.accumulate);
+	}
+}
+
+// `v` where it lies if the product can read it there, else act(v) copied to the workspace.
+template <class T>
+static Matrix operand(const Kept<T>& v, int act, size_t rows, uint32_t width, Room& room, hipStream_t s) {
+	if (v.v && v.wide && act == NGP_ACT_NONE && width % 8 == 0) return {v.v, v.stride};
+	T* to = room.take<T>(rows * up8(width));
+	if (room.run && rows) {
+		const size_t blocks = (rows * (up8(width) / 8) + 255) / 256;
+		k_lay_out<T><<<(uint32_t)std::min<size_t>(blocks, 16384), 256, 0, s>>>(v, act, rows, width, to);
+		NGP_HIP_CHECK(hipGetLastError());
+	}
+	return {to, up8(width)};
+}
+
+template <class T>
+static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) {
+	Room room{static_cast<char*>(a.workspace), run};
+	if (!a.n) return 0;
+	const Matrix x = operand<T>(kept<T>(a.x, a.x_stride, {}), NGP_ACT_NONE, a.n, a.n_in, room, s);
+	const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
+	const ForwardOut<T> out{a.bias, static_cast<const T*>(a.residual), static_cast<T*>(a.y), static_cast<T*>(a.z), a.z8,
+	                        a.residual_stride, a.y_stride, a.z_stride, a.activation,
+	                        wide_rows(a.residual, a.residual_stride, 2), wide_rows(a.y, a.y_stride, 2), wide_rows(a.z, a.z_stride, 2),
+	                        wide_rows(a.z8.q, a.z8.q_stride, 1, 8)};
+	product<T, ForwardOut<T>, false, false>(x, w, a.n, a.n_out, a.n_in, out, room, s);
+	return room.bytes;
+}
+
+template <class T>
+static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipStream_t s) {
+	Room room{static_cast<char*>(a.workspace), run};
+	const bool products = a.dx || a.dweights, active = a.activation != NGP_ACT_NONE;
+	const Kept<T> dy = kept<T>(a.dy, a.dy_stride, {}), x = kept<T>(a.x, a.x_stride, a.x8);
+	// dz where it has to be made, or copied into rows that the products can read
+	const bool make_dz = products && (active || !dy.wide || a.n_out % 8);
+	T* dz_to = make_dz ? room.take<T>((size_t)a.n * up8(a.n_out)) : nullptr;
+	const Matrix dz = make_dz ? Matrix{dz_to, up8(a.n_out)} : Matrix{a.dy, a.dy_stride};
+	if (make_dz || a.dbias) {
+		// every workgroup takes 32 rows at least; about four workgroups per CU
+		uint32_t groups = 1;
+		while (groups < 32 && groups * 8 < a.n_out) groups *= 2;
+		const uint32_t wide = (a.n_out + groups * 8 - 1) / (groups * 8), lines = 256 / groups;
+		const uint32_t shares = (uint32_t)std::max<size_t>(1, std::min<size_t>((a.n + lines - 1) / lines, std::max(1u, 1024u / wide)));
+		const size_t each = ((size_t)a.n + shares - 1) / shares;
+		float* part = a.dbias ? room.take<float>((size_t)shares * a.n_out) : nullptr;
+		if (run) {
+			k_linear_dz<T><<<dim3(wide, shares), 256, 0, s>>>(dy, kept<T>(a.z, a.z_stride, a.z8), a.activation, a.n, a.n_out, groups, each,
+			                                                 dz_to, part);
 			NGP_HIP_CHECK(hipGetLastError());
+			if (a.dbias) {
+				k_column_sum<<<(a.n_out + 15) / 16, 256, 0, s>>>(part, shares, a.n_out, a.dbias, a.accumulate);
+				NGP_HIP_CHECK(hipGetLastError());
+			}
 		}
 	}
-	const Kept<T> x = kept<T>(a.x, a.x_stride, a.x8);
 	if (a.dx && a.n) {
-		Operand<T> w{Kept<T>{static_cast<const T*>(a.weights), a.weights_stride}};
-		w.by_k = true;
-		const GradientOut<T> out{static_cast<T*>(a.dx), a.dx_stride, x, a.x_activation, {}};
-		k_product<T><<<dim3((a.n + TILE - 1) / TILE, (a.n_in + TILE - 1) / TILE), 256, 0, s>>>(dz, w, a.n, a.n_in, a.n_out, out);
-		NGP_HIP_CHECK(hipGetLastError());
+		const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
+		const GradientOut<T> out{static_cast<T*>(a.dx), a.dx_stride, x, a.x_activation, wide_rows(a.dx, a.dx_stride, 2)};
+		product<T, GradientOut<T>, false, true>(dz, w, a.n, a.n_in, a.n_out, out, room, s);
 	}
 	if (a.dweights) {
-		dz.by_k = true;
-		Operand<T> xs{x, a.x_activation, true};
-		const WeightsOut<T> out{a.dweights, a.dweights_stride, a.dweights_type == NGP_TYPE_F32, a.accumulate, {}};
-		k_product<T><<<dim3((a.n_out + TILE - 1) / TILE, (a.n_in + TILE - 1) / TILE), 256, 0, s>>>(dz, xs, a.n_out, a.n_in, a.n, out);
-		NGP_HIP_CHECK(hipGetLastError());
+		const Matrix xs = operand<T>(x, a.x_activation, a.n, a.n_in, room, s);
+		const bool f32 = a.dweights_type == NGP_TYPE_F32;
+		const WeightsOut<T> out{a.dweights, a.dweights_stride, f32, a.accumulate != 0, wide_rows(a.dweights, a.dweights_stride, f32 ? 4 : 2)};
+		product<T, WeightsOut<T>, true, true>(dz, xs, a.n_out, a.n_in, a.n, out, room, s);
 	}
+	return room.bytes;
+}
+
+size_t linear_workspace(const ngp_linear_args& a) {
+	return a.type == NGP_TYPE_F16 ? linear_forward<f16>(a, false, 0) : linear_forward<bf16>(a, false, 0);
+}
+size_t linear_backward_workspace(const ngp_linear_backward_args& a) {
+	return a.type == NGP_TYPE_F16 ? linear_backward<f16>(a, false, 0) : linear_backward<bf16>(a, false, 0);
 }
 
 void run_linear_forward(const ngp_linear_args& a, hipStream_t s) {
-	if (a.type == NGP_TYPE_F16) linear_forward<f16>(a, s);
-	else linear_forward<bf16>(a, s);
+	if (a.type == NGP_TYPE_F16) linear_forward<f16>(a, true, s);
+	else linear_forward<bf16>(a, true, s);
 }
 
 void run_linear_backward(const ngp_linear_backward_args& a, hipStream_t s) {
-	if (a.type == NGP_TYPE_F16) linear_backward<f16>(a, s);
-	else linear_backward<bf16>(a, s);
+	if (a.type == NGP_TYPE_F16) linear_backward<f16>(a, true, s);
+	else linear_backward<bf16>(a, true, s);
 }
 
 }  // namespace ngp
