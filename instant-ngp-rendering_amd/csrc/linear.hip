@@ -14,6 +14,7 @@
 
 namespace ngp {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -195,6 +196,24 @@ struct Fragments {
 	}
 };
 
+// Eight neighbouring columns of C (j a multiple of 8, `left` of them and more up to the row's end; 0: none) to the caller's
+// matrices.  The four lanes of a block of 32 call it together.
+template <class T, class Out>
+__device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t j, uint32_t left, float (&v)[8]) {
+	float z[8] = {};
+	if (left) out.finish(i, j, left, v, z);
+	if (!out.z8.q) return;
+	uint32_t top = 0;
+#pragma unroll
+	for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left ? magnitude_bits(z[k]) : 0u);
+	top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+	top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+	if (!left) return;
+	const uint32_t scale = checkpoint_scale<T>(top);
+	checkpoint_store8(out.z8.q + i * out.z8.q_stride + j, left, out.z8_wide, scale, z);
+	if (j % 32u == 0) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
+}
+
 // BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through two LDS buffers: while the matrix cores
 // work on one stage, the next is on its way from memory into the other buffer without passing registers.  P's rows are
 // the matrix instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
@@ -271,48 +290,38 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) 
 		}
 	}
 
-	// register r of a 32 x 32 tile: column r % 4 + 8 (r / 4) + 4 (lane / 32), row lane % 32; two groups of four columns
-	// change places between the half waves, which leaves every lane eight neighbouring ones, twice
-	const uint32_t n8 = (a.N + 7u) & ~7u;
+	// Register r of a 32 x 32 tile holds column r % 4 + 8 (r / 4) + 4 (lane / 32) of row lane % 32.  Each wave passes 32 rows
+	// at a time through LDS and takes them out again row by row, eight neighbouring columns per lane: whole lines of the
+	// caller's matrices per access, and one copy of the code that finishes a value.
+	constexpr int WN = BN / 2, PITCH = WN + 4, LANES = WN / 8;  // + 4: 32 rows' 16-byte pieces on different banks
+	static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "the stages' LDS holds the strips");
+	float* strip = reinterpret_cast<float*>(lds) + wave * 32u * PITCH;
+	const uint32_t n8 = (a.N + 7u) & ~7u, j = n0 + wn + lane % LANES * 8u;
+	__syncthreads();  // the last stage has been read
 #pragma unroll
 	for (int m = 0; m < TM; ++m) {
-		const size_t i = m0 + wm + m * 32u + (lane & 31u);
 #pragma unroll
-		for (int n = 0; n < TN; ++n) {
-			float v[2][8];
+		for (int n = 0; n < TN; ++n)
 #pragma unroll
-			for (int h = 0; h < 2; ++h)
+			for (int g = 0; g < 4; ++g)
+				*reinterpret_cast<f32x4*>(strip + (lane & 31u) * PITCH + n * 32 + g * 8 + (lane >> 5) * 4u) =
+				    f32x4{c[n][m][4 * g], c[n][m][4 * g + 1], c[n][m][4 * g + 2], c[n][m][4 * g + 3]};
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+		for (uint32_t r = lane / LANES; r < 32u; r += 64u / LANES) {
+			const size_t i = m0 + wm + m * 32u + r;
+			float v[8];
+			const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u);
+			const f32x4 hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u + 4);
 #pragma unroll
-				for (int k = 0; k < 4; ++k) {
-					const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[n][m][8 * h + k]), __float_as_uint(c[n][m][8 * h + 4 + k]),
-					                                                false, false);
-					v[h][k] = __uint_as_float(s[0]);
-					v[h][k + 4] = __uint_as_float(s[1]);
-				}
-			const uint32_t j = n0 + wn + n * 32u + 8u * (lane >> 5);
+			for (int k = 0; k < 8; ++k) v[k] = k < 4 ? lo[k & 3] : hi[k & 3];
 			if (a.splits > 1) {
-#pragma unroll
-				for (int h = 0; h < 2; ++h)
-					if (i < a.M && j + 16u * h < n8) store8(a.partial + ((size_t)split * a.M + i) * n8 + j + 16u * h, 8, true, v[h]);
+				if (i < a.M && j < n8) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, true, v);
 				continue;
 			}
-			float z[2][8] = {};
-			uint32_t left[2], top = 0;
-#pragma unroll
-			for (int h = 0; h < 2; ++h) {
-				left[h] = i < a.M && j + 16u * h < a.N ? a.N - j - 16u * h : 0u;
-				if (left[h]) out.finish(i, j + 16u * h, left[h], v[h], z[h]);
-#pragma unroll
-				for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left[h] ? magnitude_bits(z[h][k]) : 0u);
-			}
-			if (!out.z8.q) continue;
-			const auto s = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-			const uint32_t scale = checkpoint_scale<T>(max(s[0], s[1]));
-#pragma unroll
-			for (int h = 0; h < 2; ++h)
-				if (left[h]) checkpoint_store8(out.z8.q + i * out.z8.q_stride + j + 16u * h, left[h], out.z8_wide, scale, z[h]);
-			if (left[0] && lane < 32u) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
+			finish_block<T>(out, i, j, i < a.M && j < a.N ? a.N - j : 0u, v);
 		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 	}
 }
 
@@ -323,7 +332,7 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 	const size_t t = (size_t)blockIdx.x * 256u + threadIdx.x, i = t / chunks;
 	const uint32_t j = (uint32_t)(t % chunks) * 8u;
 	const bool in = i < M && j < N;
-	float v[8] = {}, z[8] = {};
+	float v[8] = {};
 	if (in)
 		for (uint32_t s = 0; s < splits; ++s) {
 			float x[8];
@@ -331,18 +340,7 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] += x[k];
 		}
-	const uint32_t left = in ? N - j : 0u;
-	if (left) out.finish(i, j, left, v, z);
-	if (!out.z8.q) return;
-	uint32_t top = 0;
-#pragma unroll
-	for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left ? magnitude_bits(z[k]) : 0u);
-	top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-	top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-	if (!left) return;
-	const uint32_t scale = checkpoint_scale<T>(top);
-	checkpoint_store8(out.z8.q + i * out.z8.q_stride + j, left, out.z8_wide, scale, z);
-	if (j % 32u == 0) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
+	finish_block<T>(out, i, j, in ? N - j : 0u, v);
 }
 
 // ---- operands that do not lie as the product wants them ---------------------------------------------------------------
