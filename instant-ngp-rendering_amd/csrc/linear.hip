@@ -135,10 +135,18 @@ struct Stage {
 	const char* base;       // of the stage's first element (uniform)
 	size_t step;            // bytes to the next stage
 	uint32_t offset[LOADS]; // a thread's chunks
-	uint32_t k_of[LOADS];   // their first k in the stage
+	__device__ static __forceinline__ uint32_t k_of(int l) {  // and their first k in the stage
+		const uint32_t c = threadIdx.x + l * PRODUCT_THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
+		return BY_K ? line : (at ^ (line & 7u)) * 8u;
+	}
 
-	// rows [row0, rows) of the matrix from k0 on
-	__device__ __forceinline__ void begin(const Matrix& m, size_t row0, size_t rows, size_t k0) {
+	size_t lines;           // [k][row]: lines of k that are left from `base` on
+	uint32_t line_bytes;
+
+	// rows [row0, rows) of the matrix, k from k0 to K
+	__device__ __forceinline__ void begin(const Matrix& m, size_t row0, size_t rows, size_t k0, size_t K) {
+		lines = K - k0;
+		line_bytes = (uint32_t)m.stride * 2u;
 		const uint32_t left = (uint32_t)min(rows - row0, (size_t)ROWS);
 		base = static_cast<const char*>(m.v) + (BY_K ? k0 * m.stride + row0 : row0 * m.stride + k0) * 2;
 		step = BY_K ? m.stride * (PRODUCT_K * 2) : PRODUCT_K * 2;
@@ -146,20 +154,34 @@ struct Stage {
 		for (int l = 0; l < LOADS; ++l) {
 			const uint32_t c = threadIdx.x + l * PRODUCT_THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
 			const uint32_t row = BY_K ? (at ^ twist(line)) * 8u : line;
-			k_of[l] = BY_K ? line : (at ^ (line & 7u)) * 8u;
-			offset[l] = row < left ? (BY_K ? k_of[l] * (uint32_t)m.stride + row : row * (uint32_t)m.stride + k_of[l]) * 2u : OUTSIDE;
+			offset[l] = row < left ? (BY_K ? line * (uint32_t)m.stride + row : row * (uint32_t)m.stride + k_of(l)) * 2u : OUTSIDE;
 		}
 	}
-	// k_left: how much of K is left from this stage on
-	__device__ __forceinline__ void load(char* lds, uint32_t k_left) {
-		const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, 0x7fffffff, 0x00027000);
+	// The first stage, of which k below `k_in` is there (the rest is zeros), then the others, which are whole but for lines
+	// past K.  Nothing is read without `more`.
+	__device__ __forceinline__ void load_first(char* lds, uint32_t k_in) {
+		uint32_t at[LOADS];
+#pragma unroll
+		for (int l = 0; l < LOADS; ++l) at[l] = k_of(l) < k_in ? offset[l] : OUTSIDE;
+		issue(lds, at, true);
+		base += (BY_K ? step / PRODUCT_K : 2) * k_in;
+		lines -= min((size_t)k_in, lines);
+	}
+	__device__ __forceinline__ void load(char* lds, bool more) {
+		issue(lds, offset, more);
+		base += step;
+		lines -= min((size_t)PRODUCT_K, lines);
+	}
+	__device__ __forceinline__ void issue(char* lds, const uint32_t (&at)[LOADS], bool more) {
+		// the buffer's end, past which a load gives zeros: after the last line of k, or nowhere
+		const uint32_t end = !more ? 0u : (BY_K ? (uint32_t)min((size_t)PRODUCT_K, lines) * line_bytes : 0x7fffffffu);
+#ifdef __HIP_DEVICE_COMPILE__  // (with this builtin in them the compiler's host pass leaves out some of the kernels' stubs)
+		const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)end, 0x00027000);
 		char* wave = lds + (threadIdx.x & ~63u) * 16u;
 #pragma unroll
-		for (int l = 0; l < LOADS; ++l) {
-			const uint32_t at = k_of[l] < k_left ? offset[l] : OUTSIDE;
-			__builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(wave + l * PRODUCT_THREADS * 16), 16, at, 0, 0, 0);
-		}
-		base += step;
+		for (int l = 0; l < LOADS; ++l)
+			__builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(wave + l * PRODUCT_THREADS * 16), 16, at[l], 0, 0, 0);
+#endif
 	}
 };
 
@@ -195,6 +217,19 @@ struct Fragments {
 		}
 	}
 };
+
+// Asks the compiler's scheduler for an even mixture of the LDS reads, the loads and the matrix instructions that stand
+// before it, instead of one kind after the other.
+template <int READS, int LOADS, int PRODUCTS>
+__device__ __forceinline__ void alternate() {
+	if constexpr (PRODUCTS > 0) {
+		constexpr int reads = (READS + PRODUCTS - 1) / PRODUCTS, loads = (LOADS + PRODUCTS - 1) / PRODUCTS;
+		if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+		if constexpr (loads > 0) __builtin_amdgcn_sched_group_barrier(0x010, loads, 0);
+		__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+		alternate<READS - reads, LOADS - loads, PRODUCTS - 1>();
+	}
+}
 
 // Eight neighbouring columns of C (j a multiple of 8, `left` of them and more up to the row's end; 0: none) to the caller's
 // matrices.  The four lanes of a block of 32 call it together.
@@ -237,57 +272,67 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) 
 
 	const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u;
 	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
-	const size_t k0 = split * a.k_each, k1 = min(k0 + a.k_each, a.K);
+	// rows along k are filled up to 8 with zeros; lines past K are not there, which the loads know
+	const size_t k0 = split * a.k_each, k1 = min(k0 + a.k_each, (a.K + 7u) & ~(size_t)7u);
 	const uint32_t stages = (uint32_t)((k1 - k0 + PRODUCT_K - 1) / PRODUCT_K);
 
-	PStage ps;
-	QStage qs;
-	Fragments<T, BM, P_BY_K, TM> pf;
-	Fragments<T, BN, Q_BY_K, TN> qf;
-	pf.begin(wm);
-	qf.begin(wn);
 	f32x16 c[TN][TM] = {};
 	if (stages) {
-		ps.begin(a.p, m0, a.M, k0);
-		qs.begin(a.q, n0, a.N, k0);
-		auto load = [&](uint32_t s) {
-			const uint32_t left = (uint32_t)min(k1 - k0 - (size_t)s * PRODUCT_K, (size_t)PRODUCT_K);
-			char* to = lds + (s & 1u) * STAGE;
-			ps.load(to, left);
-			qs.load(to + PStage::BYTES, left);
-		};
+		PStage ps;
+		QStage qs;
+		Fragments<T, BM, P_BY_K, TM> pf;
+		Fragments<T, BN, Q_BY_K, TN> qf;
+		ps.begin(a.p, m0, a.M, k0, a.K);
+		qs.begin(a.q, n0, a.N, k0, a.K);
+		pf.begin(wm);
+		qf.begin(wn);
+		constexpr int READS = TM * (P_BY_K ? 2 : 1) + TN * (Q_BY_K ? 2 : 1), LOADS = PStage::LOADS + QStage::LOADS;
 		s16x8 p[2][TM], q[2][TN];
-		auto read = [&](const char* from, int s) {
+		auto read = [&](const char* from, int k) {
 #pragma unroll
-			for (int t = 0; t < TN; ++t) q[s & 1][t] = qf.read(from + PStage::BYTES, s, t);
+			for (int t = 0; t < TN; ++t) q[k & 1][t] = qf.read(from + PStage::BYTES, k, t);
 #pragma unroll
-			for (int t = 0; t < TM; ++t) p[s & 1][t] = pf.read(from, s, t);
+			for (int t = 0; t < TM; ++t) p[k & 1][t] = pf.read(from, k, t);
+		};
+		auto multiply = [&](int k) {
+#pragma unroll
+			for (int n = 0; n < TN; ++n)
+#pragma unroll
+				for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k & 1][n], p[k & 1][m], c[n][m]);
 		};
 		auto arrived = [] {  // this wave's reads of the one buffer are done and its loads into the other there; then everybody's
 			__builtin_amdgcn_s_waitcnt(0);
 			__syncthreads();
 		};
-		load(0);
+		// the part of K that fills no stage comes first, so that the loop has whole stages only
+		const uint32_t k_in = (uint32_t)((k1 - k0 - 1) % PRODUCT_K) + 1u;
+		ps.load_first(lds, k_in);
+		qs.load_first(lds + PStage::BYTES, k_in);
 		arrived();
-		if (stages > 1) load(1);
+		ps.load(lds + STAGE, stages > 1);
+		qs.load(lds + STAGE + PStage::BYTES, stages > 1);
 		read(lds, 0);
-		for (uint32_t s = 0; s < stages; ++s) {
-			const char* now = lds + (s & 1u) * STAGE;
+		uint32_t now = 0;
+		for (uint32_t s = 1; s < stages; ++s, now ^= STAGE) {
 #pragma unroll
-			for (int k = 0; k < 4; ++k) {
-				if (k < 3) {
-					read(now, k + 1);
-				} else if (s + 1 < stages) {
-					arrived();
-					if (s + 2 < stages) load(s + 2);
-					read(lds + ((s + 1) & 1u) * STAGE, 0);
-				}
-#pragma unroll
-				for (int n = 0; n < TN; ++n)
-#pragma unroll
-					for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k & 1][n], p[k & 1][m], c[n][m]);
+			for (int k = 0; k < 3; ++k) {
+				read(lds + now, k + 1);
+				multiply(k);
+				alternate<READS, 0, TM * TN>();
 			}
+			arrived();
+			ps.load(lds + now, s + 1 < stages);
+			qs.load(lds + now + PStage::BYTES, s + 1 < stages);
+			read(lds + (now ^ STAGE), 0);
+			multiply(3);
+			alternate<READS, LOADS, TM * TN>();
 		}
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			if (k < 3) read(lds + now, k + 1);
+			multiply(k);
+		}
+		__builtin_amdgcn_s_waitcnt(0);
 	}
 
 	// Register r of a 32 x 32 tile holds column r % 4 + 8 (r / 4) + 4 (lane / 32) of row lane % 32.  Each wave passes 32 rows
