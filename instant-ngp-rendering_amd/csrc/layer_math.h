@@ -21,15 +21,16 @@ __device__ __forceinline__ T narrow(float v) { return (T)v; }  // to nearest, ti
 
 // A value of NGP_ACT_* and its derivative.  exp is the hardware's 2^x (v_exp_f32, ~1 ulp) of x log2(e) rounded once:
 // relative error below 2^-23 (1 + |x|), against the half step 2^-12 / 2^-9 of the 16-bit results.
-__device__ __forceinline__ float act_exp(float x) { return __expf(x); }
+__device__ __forceinline__ float act_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 __device__ __forceinline__ float act_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// The normal distribution: Phi(z) and exp(-z^2 / 2).  The lower tail Phi(-a) = exp(-a^2 / 2) R(a), R the scaled
-// complementary error function (half of it), here t P(t) with t = 1 / (1 + 0.31 a) and P the degree-5 polynomial that was
-// fitted to it over 0 <= a <= 14 for the least largest relative error: 4.8e-6.
-__device__ __forceinline__ float normal_cdf(float z, float& bell) {
-	const float a = fabsf(z);
-	bell = act_exp(-0.5f * z * z);
+// The normal distribution's tail Phi(-a), a = min(|z|, 20) (nothing of a float's tail is left there), and exp(-z^2 / 2).
+// Phi(-a) = exp(-a^2 / 2) R(a), R the scaled complementary error function (half of it), here t P(t) with
+// t = 1 / (1 + 0.31 a) and P the degree-5 polynomial that was fitted to it over 0 <= a <= 14 for the least largest
+// relative error: 4.8e-6.
+__device__ __forceinline__ float normal_tail(float z, float& a, float& bell) {
+	a = fminf(fabsf(z), 20.0f);
+	bell = __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);  // -log2(e) / 2
 	const float t = act_rcp(__builtin_fmaf(0.31f, a, 1.0f));
 	float p = -0.0739346937707959f;
 	p = __builtin_fmaf(p, t, 0.18046493448939863f);
@@ -37,17 +38,19 @@ __device__ __forceinline__ float normal_cdf(float z, float& bell) {
 	p = __builtin_fmaf(p, t, 0.13343541794249958f);
 	p = __builtin_fmaf(p, t, 0.12044041920221424f);
 	p = __builtin_fmaf(p, t, 0.12386071695430309f);
-	const float tail = bell * t * p;
-	return z < 0.0f ? tail : 1.0f - tail;
+	return bell * (t * p);
 }
 
 __device__ __forceinline__ float act_value(int act, float z) {
-	float bell;
 	switch (act) {
 		case NGP_ACT_RELU: return z <= 0.0f ? 0.0f : z;  // a NaN stays one
 		case NGP_ACT_LOGISTIC: return act_rcp(1.0f + act_exp(-z));
 		case NGP_ACT_EXPONENTIAL: return act_exp(z);
-		case NGP_ACT_GELU: return z * normal_cdf(z, bell);
+		case NGP_ACT_GELU: {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+			float a, bell;
+			const float tail = normal_tail(z, a, bell);
+			return __builtin_fmaf(-a, tail, fmaxf(z, 0.0f));
+		}
 		case NGP_ACT_SILU: return z * act_rcp(1.0f + act_exp(-z));
 		default: return z;
 	}
@@ -62,9 +65,9 @@ __device__ __forceinline__ float act_slope(int act, float z) {
 		}
 		case NGP_ACT_EXPONENTIAL: return act_exp(z);
 		case NGP_ACT_GELU: {
-			float bell;
-			const float c = normal_cdf(z, bell);
-			return __builtin_fmaf(z * 0.3989422804014327f, bell, c);
+			float a, bell;
+			const float tail = normal_tail(z, a, bell);
+			return __builtin_fmaf(z * 0.3989422804014327f, bell, z < 0.0f ? tail : 1.0f - tail);
 		}
 		case NGP_ACT_SILU: {
 			const float s = act_rcp(1.0f + act_exp(-z));
@@ -101,15 +104,18 @@ __device__ __forceinline__ void act_slopes(int act, float (&v)[8]) {
 template <class T>
 using v8 = T __attribute__((ext_vector_type(8), aligned(16)));
 template <class T>
+__device__ __forceinline__ v8<T> load8_raw(const T* p, uint32_t left, bool wide) {
+	if (wide && left >= 8) return *reinterpret_cast<const v8<T>*>(p);
+	v8<T> x;
+#pragma unroll
+	for (int k = 0; k < 8; ++k) x[k] = (uint32_t)k < left ? p[k] : narrow<T>(0.0f);
+	return x;
+}
+template <class T>
 __device__ __forceinline__ void load8(const T* p, uint32_t left, bool wide, float (&v)[8]) {
-	if (wide && left >= 8) {
-		const v8<T> x = *reinterpret_cast<const v8<T>*>(p);
+	const v8<T> x = load8_raw(p, left, wide);
 #pragma unroll
-		for (int k = 0; k < 8; ++k) v[k] = widen(x[k]);
-	} else {
-#pragma unroll
-		for (int k = 0; k < 8; ++k) v[k] = (uint32_t)k < left ? widen(p[k]) : 0.0f;
-	}
+	for (int k = 0; k < 8; ++k) v[k] = widen(x[k]);
 }
 template <class T>
 __device__ __forceinline__ void store8(T* p, uint32_t left, bool wide, const float (&v)[8]) {
@@ -143,11 +149,21 @@ __device__ __forceinline__ float checkpoint_value(int q, uint32_t scale) {
 	return scale == 255u ? __uint_as_float(0x7fc00000u) : ldexpf((float)q, (int)scale - 133);
 }
 
-// Eight neighbouring values of one block (the first at a multiple of 8) to and from a checkpoint's row.
+// Eight neighbouring values of one block (the first at a multiple of 8) to and from a checkpoint's row.  Adding 1.5 2^23
+// rounds to the nearest integer, ties to even, and leaves it in the sum's low bits.
 __device__ __forceinline__ void checkpoint_store8(int8_t* q, uint32_t left, bool wide, uint32_t scale, const float (&v)[8]) {
-	uint32_t w[2] = {0, 0};
+	const int power = 133 - (int)scale;
+	uint32_t w[2];
 #pragma unroll
-	for (int k = 0; k < 8; ++k) w[k / 4] |= ((uint32_t)checkpoint_q(v[k], scale) & 0xffu) << (8 * (k % 4));
+	for (int h = 0; h < 2; ++h) {
+		uint32_t b[4];
+#pragma unroll
+		for (int k = 0; k < 4; ++k)
+			b[k] = __float_as_uint(__builtin_amdgcn_fmed3f(ldexpf(v[4 * h + k], power), -127.0f, 127.0f) + 12582912.0f);
+		// bytes 0 of two, then of all four
+		const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+		w[h] = scale == 255u ? 0u : lo | hi;
+	}
 	if (wide && left >= 8) {
 		*reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
 	} else {
@@ -156,15 +172,23 @@ __device__ __forceinline__ void checkpoint_store8(int8_t* q, uint32_t left, bool
 			if ((uint32_t)k < left) q[k] = (int8_t)(w[k / 4] >> (8 * (k % 4)));
 	}
 }
-__device__ __forceinline__ void checkpoint_load8(const int8_t* q, uint32_t left, bool wide, uint32_t scale, float (&v)[8]) {
-	if (wide && left >= 8) {
-		const uint2 w = *reinterpret_cast<const uint2*>(q);
+__device__ __forceinline__ uint2 checkpoint_load8_raw(const int8_t* q, uint32_t left, bool wide) {
+	if (wide && left >= 8) return *reinterpret_cast<const uint2*>(q);
+	uint32_t w[2] = {0, 0};
 #pragma unroll
-		for (int k = 0; k < 8; ++k) v[k] = checkpoint_value((int8_t)((k < 4 ? w.x : w.y) >> (8 * (k % 4))), scale);
-	} else {
+	for (int k = 0; k < 8; ++k)
+		if ((uint32_t)k < left) w[k / 4] |= (uint32_t)(uint8_t)q[k] << (8 * (k % 4));
+	return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void checkpoint_widen8(uint2 w, uint32_t scale, float (&v)[8]) {
 #pragma unroll
-		for (int k = 0; k < 8; ++k) v[k] = (uint32_t)k < left ? checkpoint_value(q[k], scale) : 0.0f;
-	}
+	for (int k = 0; k < 8; ++k) v[k] = checkpoint_value((int8_t)((k < 4 ? w.x : w.y) >> (8 * (k % 4))), scale);
+}
+
+// The largest of four neighbouring lanes' (lanes 4 k .. 4 k + 3).
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+	x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
+	return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
 }
 
 // Activations as a backward pass finds them: [rows][stride] of T, or a checkpoint (v null), or absent (both null).
@@ -176,10 +200,30 @@ struct Kept {
 	const uint8_t* scale = nullptr;
 	size_t q_stride = 0, scale_stride = 0;
 	bool wide = false;  // rows start on 16 bytes (a checkpoint's: on 8)
-	__device__ __forceinline__ void at8(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const {
-		if (v) load8(v + i * stride + j, left, wide, x);
-		else checkpoint_load8(q + i * q_stride + j, left, wide, scale[i * scale_stride + (j >> 5)], x);
+	struct Raw {  // eight neighbouring values as they lie: of T, or eight q and their scale
+		v8<T> v;
+		uint2 q;
+		uint32_t scale;
+	};
+	__device__ __forceinline__ Raw raw8(size_t i, uint32_t j, uint32_t left) const {
+		Raw r = {};
+		if (v) {
+			r.v = load8_raw(v + i * stride + j, left, wide);
+		} else {
+			r.q = checkpoint_load8_raw(q + i * q_stride + j, left, wide);
+			r.scale = scale[i * scale_stride + (j >> 5)];
+		}
+		return r;
 	}
+	__device__ __forceinline__ void widen8(const Raw& r, float (&x)[8]) const {
+		if (v) {
+#pragma unroll
+			for (int k = 0; k < 8; ++k) x[k] = widen(r.v[k]);
+		} else {
+			checkpoint_widen8(r.q, r.scale, x);
+		}
+	}
+	__device__ __forceinline__ void at8(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const { widen8(raw8(i, j, left), x); }
 };
 
 inline bool wide_rows(const void* p, size_t stride, size_t element, size_t bytes = 16) {

@@ -28,6 +28,7 @@ __device__ __forceinline__ f32x16 mfma(bf16, s16x8 a, s16x8 b, f32x16 c) {
 }
 
 // ---- what a product does with its fp32 sums, eight neighbouring columns of a row at a time --------------------------
+// Columns: what the rows share; Fetched: what is read for a row's eight, asked for before any of them is finished.
 template <class T>
 struct ForwardOut {
 	const float* bias;
@@ -38,18 +39,32 @@ struct ForwardOut {
 	size_t residual_stride, y_stride, z_stride;
 	int act;
 	bool residual_wide, y_wide, z_wide, z8_wide;
-	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, float (&v)[8], float (&kept)[8]) const {
+	struct Columns {
+		float bias[8];
+	};
+	struct Fetched {
+		v8<T> r;
+	};
+	__device__ __forceinline__ Columns columns(uint32_t j, uint32_t left) const {
+		Columns c;
 #pragma unroll
-		for (int k = 0; k < 8; ++k) v[k] += bias && (uint32_t)k < left ? bias[j + k] : 0.0f;
+		for (int k = 0; k < 8; ++k) c.bias[k] = bias && (uint32_t)k < left ? bias[j + k] : 0.0f;
+		return c;
+	}
+	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
+		Fetched f = {};
+		if (residual) f.r = load8_raw(residual + i * residual_stride + j, left, residual_wide);
+		return f;
+	}
+	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns& c, const Fetched& f, float (&v)[8],
+	                                       float (&kept)[8]) const {
 #pragma unroll
-		for (int k = 0; k < 8; ++k) kept[k] = v[k];
+		for (int k = 0; k < 8; ++k) kept[k] = v[k] += c.bias[k];
 		if (z) store8(z + i * z_stride + j, left, z_wide, v);
 		act_values(act, v);
 		if (residual) {
-			float r[8];
-			load8(residual + i * residual_stride + j, left, residual_wide, r);
 #pragma unroll
-			for (int k = 0; k < 8; ++k) v[k] += r[k];
+			for (int k = 0; k < 8; ++k) v[k] += widen(f.r[k]);
 		}
 		store8(y + i * y_stride + j, left, y_wide, v);
 	}
@@ -64,10 +79,17 @@ struct GradientOut {  // dx
 	bool wide;
 	static constexpr ngp_checkpoint8 z8 = {};
 	static constexpr bool z8_wide = false;
-	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, float (&v)[8], float (&)[8]) const {
+	struct Columns {};
+	typedef typename Kept<T>::Raw Fetched;
+	__device__ __forceinline__ Columns columns(uint32_t, uint32_t) const { return {}; }
+	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
+		return act == NGP_ACT_NONE ? Fetched{} : p.raw8(i, j, left);
+	}
+	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns&, const Fetched& f, float (&v)[8],
+	                                       float (&)[8]) const {
 		if (act != NGP_ACT_NONE) {
 			float s[8];
-			p.at8(i, j, left, s);
+			p.widen8(f, s);
 			act_slopes(act, s);
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] *= s[k];
@@ -83,16 +105,22 @@ struct WeightsOut {  // dW
 	bool f32, accumulate, wide;
 	static constexpr ngp_checkpoint8 z8 = {};
 	static constexpr bool z8_wide = false;
-	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, float (&v)[8], float (&)[8]) const {
+	struct Columns {};
+	struct Fetched {
+		float before[8];
+	};
+	__device__ __forceinline__ Columns columns(uint32_t, uint32_t) const { return {}; }
+	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
+		Fetched f = {};
+		if (accumulate) load8(static_cast<const float*>(dw) + i * stride + j, left, wide, f.before);
+		return f;
+	}
+	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns&, const Fetched& f, float (&v)[8],
+	                                       float (&)[8]) const {
 		if (f32) {
-			float* d = static_cast<float*>(dw) + i * stride + j;
-			if (accumulate) {
-				float o[8];
-				load8(d, left, wide, o);
 #pragma unroll
-				for (int k = 0; k < 8; ++k) v[k] += o[k];
-			}
-			store8(d, left, wide, v);
+			for (int k = 0; k < 8; ++k) v[k] += f.before[k];
+			store8(static_cast<float*>(dw) + i * stride + j, left, wide, v);
 		} else {
 			store8(static_cast<T*>(dw) + i * stride + j, left, wide, v);
 		}
@@ -234,15 +262,15 @@ __device__ __forceinline__ void alternate() {
 // Eight neighbouring columns of C (j a multiple of 8, `left` of them and more up to the row's end; 0: none) to the caller's
 // matrices.  The four lanes of a block of 32 call it together.
 template <class T, class Out>
-__device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t j, uint32_t left, float (&v)[8]) {
+__device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t j, uint32_t left, const typename Out::Columns& columns,
+                                             const typename Out::Fetched& fetched, float (&v)[8]) {
 	float z[8] = {};
-	if (left) out.finish(i, j, left, v, z);
+	if (left) out.finish(i, j, left, columns, fetched, v, z);
 	if (!out.z8.q) return;
 	uint32_t top = 0;
 #pragma unroll
 	for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left ? magnitude_bits(z[k]) : 0u);
-	top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-	top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+	top = quad_max(top);
 	if (!left) return;
 	const uint32_t scale = checkpoint_scale<T>(top);
 	checkpoint_store8(out.z8.q + i * out.z8.q_stride + j, left, out.z8_wide, scale, z);
@@ -342,6 +370,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) 
 	static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "the stages' LDS holds the strips");
 	float* strip = reinterpret_cast<float*>(lds) + wave * 32u * PITCH;
 	const uint32_t n8 = (a.N + 7u) & ~7u, j = n0 + wn + lane % LANES * 8u;
+	const auto columns = out.columns(j, j < a.N ? a.N - j : 0u);
 	__syncthreads();  // the last stage has been read
 #pragma unroll
 	for (int m = 0; m < TM; ++m) {
@@ -352,19 +381,30 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) 
 				*reinterpret_cast<f32x4*>(strip + (lane & 31u) * PITCH + n * 32 + g * 8 + (lane >> 5) * 4u) =
 				    f32x4{c[n][m][4 * g], c[n][m][4 * g + 1], c[n][m][4 * g + 2], c[n][m][4 * g + 3]};
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		// four rows' reads are on their way before the first of them is worked on: the wave has its SIMD to itself
+		constexpr int ROWS = 64 / LANES, AHEAD = 32 / ROWS < 4 ? 32 / ROWS : 4;
 #pragma unroll 1
-		for (uint32_t r = lane / LANES; r < 32u; r += 64u / LANES) {
-			const size_t i = m0 + wm + m * 32u + r;
-			float v[8];
-			const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u);
-			const f32x4 hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u + 4);
+		for (uint32_t r0 = lane / LANES; r0 < 32u; r0 += ROWS * AHEAD) {
+			const size_t i0 = m0 + wm + m * 32u;
+			float v[AHEAD][8];
+			typename Out::Fetched fetched[AHEAD];
+			uint32_t left[AHEAD];
 #pragma unroll
-			for (int k = 0; k < 8; ++k) v[k] = k < 4 ? lo[k & 3] : hi[k & 3];
-			if (a.splits > 1) {
-				if (i < a.M && j < n8) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, true, v);
-				continue;
+			for (int u = 0; u < AHEAD; ++u) {
+				const uint32_t r = r0 + u * ROWS;
+				const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u);
+				const f32x4 hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u + 4);
+#pragma unroll
+				for (int k = 0; k < 8; ++k) v[u][k] = k < 4 ? lo[k & 3] : hi[k & 3];
+				left[u] = i0 + r < a.M && j < a.N ? a.N - j : 0u;
+				if (left[u] && a.splits == 1) fetched[u] = out.fetch(i0 + r, j, left[u]);
 			}
-			finish_block<T>(out, i, j, i < a.M && j < a.N ? a.N - j : 0u, v);
+#pragma unroll
+			for (int u = 0; u < AHEAD; ++u) {
+				const size_t i = i0 + r0 + u * ROWS;
+				if (a.splits == 1) finish_block<T>(out, i, j, left[u], columns, fetched[u], v[u]);
+				else if (left[u]) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, true, v[u]);
+			}
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 	}
@@ -385,7 +425,10 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] += x[k];
 		}
-	finish_block<T>(out, i, j, in ? N - j : 0u, v);
+	const uint32_t left = in ? N - j : 0u;
+	typename Out::Fetched fetched = {};
+	if (left) fetched = out.fetch(i, j, left);
+	finish_block<T>(out, i, j, left, out.columns(j, left), fetched, v);
 }
 
 // ---- operands that do not lie as the product wants them ---------------------------------------------------------------
