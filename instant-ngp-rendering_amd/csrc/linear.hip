@@ -18,6 +18,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 __device__ __forceinline__ f32x16 mfma(f16, s16x8 a, s16x8 b, f32x16 c) {
@@ -141,31 +142,33 @@ struct ProductArgs {
 	float* partial;       // [splits][M][N up to 8] where splits > 1
 };
 
-constexpr int PRODUCT_K = 64;   // of K per stage
-constexpr int PRODUCT_THREADS = 256;
+constexpr int PRODUCT_K = 64;  // splits of K are multiples of it
+constexpr int PRODUCT_THREADS = 256, WIDE_THREADS = 512;
 
-// One stage of an operand in LDS: ROWS x 64 elements of 16 bits.  Each wave's load puts 64 chunks of 16 bytes one after
-// another (buffer_load ... lds takes no other order), so rows are spread over the banks by what each lane fetches:
-//  * [row][k] in memory: 128 bytes per row, chunk c of row r holds k chunk c ^ (r & 7); ds_read_b128 of 32 rows' same
+// One stage of an operand in LDS: ROWS x DEEP (64 or 32) elements of 16 bits.  Each wave's load puts 64 chunks of 16 bytes
+// one after another (buffer_load ... lds takes no other order), so rows are spread over the banks by what each lane fetches:
+//  * [row][k] in memory: 2 DEEP bytes per row, chunk c of row r holds k chunk c ^ twist(r); ds_read_b128 of 32 rows' same
 //    k chunk touches every bank equally.
 //  * [k][row] in memory: 2 ROWS bytes per k, chunk c of line k holds rows' chunk c ^ twist(k); ds_read_b64_tr_b16 reads
 //    four k lines x 64 bytes per half wave, which the twist puts on different banks.
-template <class T, int ROWS, bool BY_K>
+template <class T, int ROWS, bool BY_K, int DEEP, int THREADS>
 struct Stage {
-	static constexpr int BYTES = ROWS * PRODUCT_K * 2;
-	static constexpr int LOADS = BYTES / 16 / PRODUCT_THREADS;
-	static constexpr int LINE = BY_K ? ROWS * 2 : PRODUCT_K * 2;  // bytes
-	static constexpr uint32_t OUTSIDE = 0xfffffff0u;              // past every buffer: the load gives zeros
-	__device__ static __forceinline__ uint32_t twist(uint32_t k) {
-		return LINE >= 256 ? ((k & 3u) << 2) | (k & 2u) : (((k >> 1) & 1u) << 2) | ((k & 1u) << 1);
+	static constexpr int BYTES = ROWS * DEEP * 2;
+	static constexpr int LOADS = BYTES / 16 / THREADS;
+	static constexpr int LINE = BY_K ? ROWS * 2 : DEEP * 2;  // bytes
+	static constexpr uint32_t OUTSIDE = 0xfffffff0u;         // past every buffer: the load gives zeros
+	static_assert(BYTES % (16 * THREADS) == 0, "every thread loads the same number of chunks");
+	__device__ static __forceinline__ uint32_t twist(uint32_t line) {
+		if constexpr (!BY_K) return LINE >= 128 ? (line >> 1) & 7u : (line >> 2) & 3u;
+		return LINE >= 256 ? ((line & 3u) << 2) | (line & 2u) : (((line >> 1) & 1u) << 2) | ((line & 1u) << 1);
 	}
 
 	const char* base;       // of the stage's first element (uniform)
 	size_t step;            // bytes to the next stage
 	uint32_t offset[LOADS]; // a thread's chunks
 	__device__ static __forceinline__ uint32_t k_of(int l) {  // and their first k in the stage
-		const uint32_t c = threadIdx.x + l * PRODUCT_THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
-		return BY_K ? line : (at ^ (line & 7u)) * 8u;
+		const uint32_t c = threadIdx.x + l * THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
+		return BY_K ? line : (at ^ twist(line)) * 8u;
 	}
 
 	size_t lines;           // [k][row]: lines of k that are left from `base` on
@@ -177,10 +180,10 @@ struct Stage {
 		line_bytes = (uint32_t)m.stride * 2u;
 		const uint32_t left = (uint32_t)min(rows - row0, (size_t)ROWS);
 		base = static_cast<const char*>(m.v) + (BY_K ? k0 * m.stride + row0 : row0 * m.stride + k0) * 2;
-		step = BY_K ? m.stride * (PRODUCT_K * 2) : PRODUCT_K * 2;
+		step = BY_K ? m.stride * (DEEP * 2) : DEEP * 2;
 #pragma unroll
 		for (int l = 0; l < LOADS; ++l) {
-			const uint32_t c = threadIdx.x + l * PRODUCT_THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
+			const uint32_t c = threadIdx.x + l * THREADS, line = c / (LINE / 16), at = c % (LINE / 16);
 			const uint32_t row = BY_K ? (at ^ twist(line)) * 8u : line;
 			offset[l] = row < left ? (BY_K ? line * (uint32_t)m.stride + row : row * (uint32_t)m.stride + k_of(l)) * 2u : OUTSIDE;
 		}
@@ -192,31 +195,35 @@ struct Stage {
 #pragma unroll
 		for (int l = 0; l < LOADS; ++l) at[l] = k_of(l) < k_in ? offset[l] : OUTSIDE;
 		issue(lds, at, true);
-		base += (BY_K ? step / PRODUCT_K : 2) * k_in;
+		base += (BY_K ? step / DEEP : 2) * k_in;
 		lines -= min((size_t)k_in, lines);
 	}
 	__device__ __forceinline__ void load(char* lds, bool more) {
 		issue(lds, offset, more);
 		base += step;
-		lines -= min((size_t)PRODUCT_K, lines);
+		lines -= min((size_t)DEEP, lines);
 	}
 	__device__ __forceinline__ void issue(char* lds, const uint32_t (&at)[LOADS], bool more) {
 		// the buffer's end, past which a load gives zeros: after the last line of k, or nowhere
-		const uint32_t end = !more ? 0u : (BY_K ? (uint32_t)min((size_t)PRODUCT_K, lines) * line_bytes : 0x7fffffffu);
-#ifdef __HIP_DEVICE_COMPILE__  // (with this builtin in them the compiler's host pass leaves out some of the kernels' stubs)
-		const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)end, 0x00027000);
-		char* wave = lds + (threadIdx.x & ~63u) * 16u;
+		const uint32_t end = !more ? 0u : (BY_K ? (uint32_t)min((size_t)DEEP, lines) * line_bytes : 0x7fffffffu);
+		const uintptr_t from = reinterpret_cast<uintptr_t>(base);
+		const i32x4 rsrc = {(int)(uint32_t)from, (int)(uint32_t)(from >> 32), (int)end, 0x00027000};
+		const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_ptr)lds) + (threadIdx.x & ~63u) * 16u);
+		// not the builtin: the compiler then waits for every load into LDS before each transposed read from it, whichever
+		// buffer they are for.  The waits are written out where the stages change; nothing is loaded into registers here, and
+		// m0 (the LDS address, a register the compiler only ever sets right before it needs it) is set in the same block.
 #pragma unroll
 		for (int l = 0; l < LOADS; ++l)
-			__builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(wave + l * PRODUCT_THREADS * 16), 16, at[l], 0, 0, 0);
-#endif
+			asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+			             :
+			             : "s"(to + l * THREADS * 16), "v"(at[l]), "s"(rsrc));
 	}
 };
 
 // A wave's 32 x 16 fragments of a stage: lane l holds row l % 32 and k = 8 (l / 32) .. + 7 of each 16.
-template <class T, int ROWS, bool BY_K, int TILES>
+template <class Stage, int ROWS, bool BY_K, int DEEP, int TILES>
 struct Fragments {
-	uint32_t offset[BY_K ? TILES : 4];
+	uint32_t offset[BY_K ? TILES : DEEP / 16];
 	__device__ __forceinline__ void begin(uint32_t row0) {
 		const uint32_t lane = threadIdx.x & 63u;
 		if constexpr (BY_K) {
@@ -225,12 +232,12 @@ struct Fragments {
 #pragma unroll
 			for (int t = 0; t < TILES; ++t) {
 				const uint32_t chunk = (row0 + t * 32u + 16u * (g & 1u)) / 8u + (p >> 1);
-				offset[t] = (8u * (g >> 1) + q) * (ROWS * 2) + ((chunk ^ Stage<T, ROWS, BY_K>::twist(q)) << 4) + (p & 1u) * 8u;
+				offset[t] = (8u * (g >> 1) + q) * (ROWS * 2) + ((chunk ^ Stage::twist(q)) << 4) + (p & 1u) * 8u;
 			}
 		} else {
 #pragma unroll
-			for (int s = 0; s < 4; ++s)
-				offset[s] = (row0 + (lane & 31u)) * (PRODUCT_K * 2) + (((s * 2u + (lane >> 5)) ^ (lane & 7u)) << 4);
+			for (int s = 0; s < DEEP / 16; ++s)
+				offset[s] = (row0 + (lane & 31u)) * (DEEP * 2) + (((s * 2u + (lane >> 5)) ^ Stage::twist(lane & 31u)) << 4);
 		}
 	}
 	__device__ __forceinline__ s16x8 read(const char* lds, int s, int t) const {  // the s-th 16 of k, the t-th 32 rows
@@ -241,7 +248,7 @@ struct Fragments {
 			const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 4 * (ROWS * 2)));
 			return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 		} else {
-			return *reinterpret_cast<const s16x8*>(lds + offset[s] + t * 32 * (PRODUCT_K * 2));
+			return *reinterpret_cast<const s16x8*>(lds + offset[s] + t * 32 * (DEEP * 2));
 		}
 	}
 };
@@ -277,41 +284,101 @@ __device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t 
 	if (j % 32u == 0) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
 }
 
+// Where a workgroup works.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight tile
+// rows deep, so that its L2 holds what they share.
+template <int BM, int BN>
+struct Place {
+	uint32_t split, n0;
+	size_t m0, k0, k1;
+	__device__ __forceinline__ explicit Place(const ProductArgs& a) {
+		const uint32_t tiles = a.tiles_m * a.tiles_n, all = gridDim.x, xcd = blockIdx.x % 8u;
+		const uint32_t id = xcd * (all / 8u) + min(xcd, all % 8u) + blockIdx.x / 8u;
+		split = id / tiles;
+		const uint32_t tile = id % tiles, group = tile / (8u * a.tiles_n), first = group * 8u, deep = min(8u, a.tiles_m - first);
+		const uint32_t in_group = tile - group * 8u * a.tiles_n;
+		m0 = (size_t)(first + in_group % deep) * BM;
+		n0 = in_group / deep * BN;
+		// rows along k are filled up to 8 with zeros; lines past K are not there, which the loads know
+		k0 = split * a.k_each;
+		k1 = min(k0 + a.k_each, (a.K + 7u) & ~(size_t)7u);
+	}
+};
+
+// A wave's TN x TM tiles of 32 x 32 sums, at row i0 and column j0 of C, to where they belong.  Register r of a tile holds
+// column r % 4 + 8 (r / 4) + 4 (lane / 32) of row lane % 32.  The wave passes 32 rows at a time through its strip of LDS and
+// takes them out again row by row, eight neighbouring columns per lane: whole lines of the caller's matrices per access, and
+// one copy of the code that finishes a value.
+template <int TN>
+constexpr int STRIP = 32 * (TN * 32 + 4);  // floats; + 4: 32 rows' 16-byte pieces on different banks
+template <class T, class Out, int TM, int TN>
+__device__ __forceinline__ void write_out(const ProductArgs& a, const Out& out, uint32_t split, size_t i0, uint32_t j0, float* strip,
+                                          const f32x16 (&c)[TN][TM]) {
+	constexpr int PITCH = TN * 32 + 4, LANES = TN * 4;
+	const uint32_t lane = threadIdx.x & 63u, n8 = (a.N + 7u) & ~7u, j = j0 + lane % LANES * 8u;
+	const auto columns = out.columns(j, j < a.N ? a.N - j : 0u);
+#pragma unroll
+	for (int m = 0; m < TM; ++m) {
+#pragma unroll
+		for (int n = 0; n < TN; ++n)
+#pragma unroll
+			for (int g = 0; g < 4; ++g)
+				*reinterpret_cast<f32x4*>(strip + (lane & 31u) * PITCH + n * 32 + g * 8 + (lane >> 5) * 4u) =
+				    f32x4{c[n][m][4 * g], c[n][m][4 * g + 1], c[n][m][4 * g + 2], c[n][m][4 * g + 3]};
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		// four rows' reads are on their way before the first of them is worked on: the wave has its SIMD to itself
+		constexpr int ROWS = 64 / LANES, AHEAD = 32 / ROWS < 4 ? 32 / ROWS : 4;
+#pragma unroll 1
+		for (uint32_t r0 = lane / LANES; r0 < 32u; r0 += ROWS * AHEAD) {
+			const size_t im = i0 + m * 32u;
+			float v[AHEAD][8];
+			typename Out::Fetched fetched[AHEAD];
+			uint32_t left[AHEAD];
+#pragma unroll
+			for (int u = 0; u < AHEAD; ++u) {
+				const uint32_t r = r0 + u * ROWS;
+				const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u);
+				const f32x4 hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u + 4);
+#pragma unroll
+				for (int k = 0; k < 8; ++k) v[u][k] = k < 4 ? lo[k & 3] : hi[k & 3];
+				left[u] = im + r < a.M && j < a.N ? a.N - j : 0u;
+				if (left[u] && a.splits == 1) fetched[u] = out.fetch(im + r, j, left[u]);
+			}
+#pragma unroll
+			for (int u = 0; u < AHEAD; ++u) {
+				const size_t i = im + r0 + u * ROWS;
+				if (a.splits == 1) finish_block<T>(out, i, j, left[u], columns, fetched[u], v[u]);
+				else if (left[u]) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, true, v[u]);
+			}
+		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+	}
+}
+
 // BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through two LDS buffers: while the matrix cores
 // work on one stage, the next is on its way from memory into the other buffer without passing registers.  P's rows are
 // the matrix instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN>
-__global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) k_product(ProductArgs a, Out out) {
+__global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, Out out) {
 	constexpr int TM = BM / 64, TN = BN / 64;  // 32 x 32 tiles per wave
-	typedef Stage<T, BM, P_BY_K> PStage;
-	typedef Stage<T, BN, Q_BY_K> QStage;
+	typedef Stage<T, BM, P_BY_K, 64, PRODUCT_THREADS> PStage;
+	typedef Stage<T, BN, Q_BY_K, 64, PRODUCT_THREADS> QStage;
 	constexpr int STAGE = PStage::BYTES + QStage::BYTES;
+	static_assert(4 * STRIP<TN> * 4 <= 2 * STAGE, "the stages' LDS holds the strips");
 	extern __shared__ __attribute__((aligned(16))) char lds[];
 
-	// workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight tile rows deep, so that
-	// its L2 holds what they share
-	const uint32_t tiles = a.tiles_m * a.tiles_n, all = gridDim.x, xcd = blockIdx.x % 8u;
-	const uint32_t id = xcd * (all / 8u) + min(xcd, all % 8u) + blockIdx.x / 8u;
-	const uint32_t split = id / tiles, tile = id % tiles;
-	const uint32_t group = tile / (8u * a.tiles_n), first = group * 8u, deep = min(8u, a.tiles_m - first);
-	const uint32_t in_group = tile - group * 8u * a.tiles_n;
-	const size_t m0 = (size_t)(first + in_group % deep) * BM;
-	const uint32_t n0 = in_group / deep * BN;
-
-	const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x & 63u;
+	const Place<BM, BN> at(a);
+	const uint32_t wave = threadIdx.x / 64u;
 	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
-	// rows along k are filled up to 8 with zeros; lines past K are not there, which the loads know
-	const size_t k0 = split * a.k_each, k1 = min(k0 + a.k_each, (a.K + 7u) & ~(size_t)7u);
-	const uint32_t stages = (uint32_t)((k1 - k0 + PRODUCT_K - 1) / PRODUCT_K);
+	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + 63u) / 64u);
 
 	f32x16 c[TN][TM] = {};
 	if (stages) {
 		PStage ps;
 		QStage qs;
-		Fragments<T, BM, P_BY_K, TM> pf;
-		Fragments<T, BN, Q_BY_K, TN> qf;
-		ps.begin(a.p, m0, a.M, k0, a.K);
-		qs.begin(a.q, n0, a.N, k0, a.K);
+		Fragments<PStage, BM, P_BY_K, 64, TM> pf;
+		Fragments<QStage, BN, Q_BY_K, 64, TN> qf;
+		ps.begin(a.p, at.m0, a.M, at.k0, a.K);
+		qs.begin(a.q, at.n0, a.N, at.k0, a.K);
 		pf.begin(wm);
 		qf.begin(wn);
 		constexpr int READS = TM * (P_BY_K ? 2 : 1) + TN * (Q_BY_K ? 2 : 1), LOADS = PStage::LOADS + QStage::LOADS;
@@ -333,7 +400,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) 
 			__syncthreads();
 		};
 		// the part of K that fills no stage comes first, so that the loop has whole stages only
-		const uint32_t k_in = (uint32_t)((k1 - k0 - 1) % PRODUCT_K) + 1u;
+		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % 64u) + 1u;
 		ps.load_first(lds, k_in);
 		qs.load_first(lds + PStage::BYTES, k_in);
 		arrived();
@@ -362,52 +429,92 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, BM * BN > 128 * 128 ? 1 : 2) 
 		}
 		__builtin_amdgcn_s_waitcnt(0);
 	}
-
-	// Register r of a 32 x 32 tile holds column r % 4 + 8 (r / 4) + 4 (lane / 32) of row lane % 32.  Each wave passes 32 rows
-	// at a time through LDS and takes them out again row by row, eight neighbouring columns per lane: whole lines of the
-	// caller's matrices per access, and one copy of the code that finishes a value.
-	constexpr int WN = BN / 2, PITCH = WN + 4, LANES = WN / 8;  // + 4: 32 rows' 16-byte pieces on different banks
-	static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "the stages' LDS holds the strips");
-	float* strip = reinterpret_cast<float*>(lds) + wave * 32u * PITCH;
-	const uint32_t n8 = (a.N + 7u) & ~7u, j = n0 + wn + lane % LANES * 8u;
-	const auto columns = out.columns(j, j < a.N ? a.N - j : 0u);
 	__syncthreads();  // the last stage has been read
+	write_out<T, Out, TM, TN>(a, out, at.split, at.m0 + wm, at.n0 + wn, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
+}
+
+// 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
+// reads its next fragments and asks for a stage of K three ahead, and then they change places.  A barrier after each half
+// keeps the two sets of four waves in opposite phases; K goes in stages of 32 through four LDS buffers.
+template <class T, class Out, bool P_BY_K, bool Q_BY_K>
+__global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a, Out out) {
+	constexpr int BM = 256, BN = 256, TM = 4, TN = 2, DEEP = 32, BUFFERS = 4;
+	typedef Stage<T, BM, P_BY_K, DEEP, WIDE_THREADS> PStage;
+	typedef Stage<T, BN, Q_BY_K, DEEP, WIDE_THREADS> QStage;
+	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
+	static_assert(8 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
+	extern __shared__ __attribute__((aligned(16))) char lds[];
+
+	const Place<BM, BN> at(a);
+	const uint32_t wave = threadIdx.x / 64u;
+	const uint32_t wm = wave / 4u * 128u, wn = wave % 4u * 64u;
+	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + DEEP - 1) / DEEP);
+
+	f32x16 c[TN][TM] = {};
+	if (stages) {
+		PStage ps;
+		QStage qs;
+		Fragments<PStage, BM, P_BY_K, DEEP, TM> pf;
+		Fragments<QStage, BN, Q_BY_K, DEEP, TN> qf;
+		ps.begin(a.p, at.m0, a.M, at.k0, a.K);
+		qs.begin(a.q, at.n0, a.N, at.k0, a.K);
+		pf.begin(wm);
+		qf.begin(wn);
+		auto load = [&](uint32_t s) {
+			char* to = lds + s % BUFFERS * STAGE;
+			ps.load(to, s < stages);
+			qs.load(to + PStage::BYTES, s < stages);
+		};
+		// nothing moves over this point, in the compiler or among the waves
+		auto meet = [] {
+			asm volatile("" ::: "memory");
+			__builtin_amdgcn_sched_barrier(0);
+			__builtin_amdgcn_s_barrier();
+			__builtin_amdgcn_sched_barrier(0);
+			asm volatile("" ::: "memory");
+		};
+		// s_waitcnt with vmcnt = a wave's loads of two stages: all but the two latest stages it asked for are there; and
+		// lgkmcnt = 0: its reads are done
+		constexpr int WAIT = 2 * LOADS | 7 << 4;
+		static_assert(2 * LOADS < 16, "vmcnt's low field");
+		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % DEEP) + 1u;
+		ps.load_first(lds, k_in);
+		qs.load_first(lds + PStage::BYTES, k_in);
+		load(1);
+		load(2);
+		__builtin_amdgcn_s_waitcnt(WAIT);
+		meet();
+		if (wave >= 4u) meet();  // the second set runs half a stage behind
+		for (uint32_t s = 0; s < stages; ++s) {
+			// the buffer of stage s - 1 is free: both sets have read it, the second before the barrier just passed
+			load(s + 3);
+			const char* from = lds + s % BUFFERS * STAGE;
+			s16x8 p[2][TM], q[2][TN];
 #pragma unroll
-	for (int m = 0; m < TM; ++m) {
+			for (int k = 0; k < 2; ++k) {
 #pragma unroll
-		for (int n = 0; n < TN; ++n)
+				for (int t = 0; t < TN; ++t) q[k][t] = qf.read(from + PStage::BYTES, k, t);
 #pragma unroll
-			for (int g = 0; g < 4; ++g)
-				*reinterpret_cast<f32x4*>(strip + (lane & 31u) * PITCH + n * 32 + g * 8 + (lane >> 5) * 4u) =
-				    f32x4{c[n][m][4 * g], c[n][m][4 * g + 1], c[n][m][4 * g + 2], c[n][m][4 * g + 3]};
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-		// four rows' reads are on their way before the first of them is worked on: the wave has its SIMD to itself
-		constexpr int ROWS = 64 / LANES, AHEAD = 32 / ROWS < 4 ? 32 / ROWS : 4;
-#pragma unroll 1
-		for (uint32_t r0 = lane / LANES; r0 < 32u; r0 += ROWS * AHEAD) {
-			const size_t i0 = m0 + wm + m * 32u;
-			float v[AHEAD][8];
-			typename Out::Fetched fetched[AHEAD];
-			uint32_t left[AHEAD];
-#pragma unroll
-			for (int u = 0; u < AHEAD; ++u) {
-				const uint32_t r = r0 + u * ROWS;
-				const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u);
-				const f32x4 hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u + 4);
-#pragma unroll
-				for (int k = 0; k < 8; ++k) v[u][k] = k < 4 ? lo[k & 3] : hi[k & 3];
-				left[u] = i0 + r < a.M && j < a.N ? a.N - j : 0u;
-				if (left[u] && a.splits == 1) fetched[u] = out.fetch(i0 + r, j, left[u]);
+				for (int t = 0; t < TM; ++t) p[k][t] = pf.read(from, k, t);
 			}
+			// stage s + 1 has arrived as far as this wave asked for it; the barriers up to its reading tell of the others
+			__builtin_amdgcn_s_waitcnt(WAIT);
+			meet();
+			__builtin_amdgcn_s_setprio(1);
 #pragma unroll
-			for (int u = 0; u < AHEAD; ++u) {
-				const size_t i = i0 + r0 + u * ROWS;
-				if (a.splits == 1) finish_block<T>(out, i, j, left[u], columns, fetched[u], v[u]);
-				else if (left[u]) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, true, v[u]);
-			}
+			for (int k = 0; k < 2; ++k)
+#pragma unroll
+				for (int n = 0; n < TN; ++n)
+#pragma unroll
+					for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k][n], p[k][m], c[n][m]);
+			__builtin_amdgcn_s_setprio(0);
+			meet();
 		}
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		if (wave < 4u) meet();
+		__builtin_amdgcn_s_waitcnt(0);
 	}
+	__syncthreads();
+	write_out<T, Out, TM, TN>(a, out, at.split, at.m0 + wm, at.n0 + wn, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
 }
 
 // The splits' sums, in their order, to where the product would have put them.
@@ -539,13 +646,12 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
 	return p;
 }
 
-template <class T, class Out, bool P_BY_K, bool Q_BY_K, int TILE>
-static void launch_product(const ProductArgs& a, const Out& out, hipStream_t s) {
-	constexpr uint32_t lds = 2 * 2 * TILE * PRODUCT_K * 2;
-	auto kernel = k_product<T, Out, P_BY_K, Q_BY_K, TILE, TILE>;
+template <class Out>
+static void launch_product(void (*kernel)(ProductArgs, Out), uint32_t threads, uint32_t lds, const ProductArgs& a, const Out& out,
+                           hipStream_t s) {
 	if (lds > 65536)
 		NGP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-	kernel<<<a.tiles_m * a.tiles_n * a.splits, PRODUCT_THREADS, lds, s>>>(a, out);
+	kernel<<<a.tiles_m * a.tiles_n * a.splits, threads, lds, s>>>(a, out);
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
@@ -557,9 +663,9 @@ static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size
 	ProductArgs a{p, q, M, K, plan.k_each, N, plan.tiles_m, plan.tiles_n, plan.splits, nullptr};
 	if (plan.splits > 1) a.partial = room.take<float>((size_t)plan.splits * M * up8(N));
 	if (!room.run) return;
-	if (plan.tile == 256) launch_product<T, Out, P_BY_K, Q_BY_K, 256>(a, out, s);
-	else if (plan.tile == 128) launch_product<T, Out, P_BY_K, Q_BY_K, 128>(a, out, s);
-	else launch_product<T, Out, P_BY_K, Q_BY_K, 64>(a, out, s);
+	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K>, WIDE_THREADS, 131072, a, out, s);
+	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128>, PRODUCT_THREADS, 65536, a, out, s);
+	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64>, PRODUCT_THREADS, 32768, a, out, s);
 	if (plan.splits > 1) {
 		const size_t items = M * ((N + 31u) / 32u * 4u);
 		k_product_join<T, Out><<<(uint32_t)((items + 255) / 256), 256, 0, s>>>(a.partial, plan.splits, M, N, out);

@@ -87,6 +87,23 @@ def test_forward(n, n_in, n_out, kind):
             check_checkpoint(z8, ze, ztol, kind)
 
 
+# enough output tiles of 256 x 256 for one per CU, with edges on both sides: each product of the passes in turn, over a K of
+# less than a stage, of whole stages, and with an odd rest
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n, n_in, n_out", [(3700, 40, 3990), (4100, 256, 3601), (3650, 3700, 16), (4001, 3520, 264), (32, 3900, 3700),
+                                            (167, 4096, 4000), (1000, 3601, 3601)])
+def test_large_products(n, n_in, n_out, kind):
+    t = U.TYPES[kind][1]
+    x, w, r = normal(1, n, n_in, t=t), normal(2, n_out, n_in, scale=n_in ** -0.5, t=t), normal(3, n, n_out, t=t)
+    z8 = U.new8(n, n_out)
+    y = U.call_linear(kind, x, w, None, "silu", r, z8=z8)
+    ze, ztol, ye, ytol = forward_reference(x, w, None, "silu", r)
+    close(y, ye, ytol + U.rounding(ye.abs() + ytol, t))
+    check_checkpoint(z8, ze, ztol, kind)
+    dy, xk, zk, w, x, z = backward_inputs(kind, n, n_in, n_out, 5, True, True)
+    check_backward(kind, U.call_linear_backward(kind, dy, xk, w, "gelu", zk, "silu"), dy, x, z, w, "gelu", "silu")
+
+
 @pytest.mark.parametrize("pad, offset", [(0, 0), (8, 0), (3, 0), (0, 1), (8, 8), (5, 3)])
 @pytest.mark.parametrize("n, n_in, n_out", [(1, 72, 40), (37, 40, 88), (70, 33, 67), (300, 200, 264)])
 def test_forward_strides_and_frames(n, n_in, n_out, pad, offset):
