@@ -99,35 +99,35 @@ __device__ __forceinline__ void act_slopes(int act, float (&v)[8]) {
 	}
 }
 
-// Eight neighbouring elements of a row that has `left` of them left, at p; one wide access where `wide` says that all
-// rows start on 16 bytes (fp32: two).
+// Eight neighbouring elements of a row that has `left` of them left, at p: one wide access wherever the row starts (global
+// memory takes 16 bytes at any address), element by element only at a row's end.
 template <class T>
-using v8 = T __attribute__((ext_vector_type(8), aligned(16)));
+using v8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 template <class T>
-__device__ __forceinline__ v8<T> load8_raw(const T* p, uint32_t left, bool wide) {
-	if (wide && left >= 8) return *reinterpret_cast<const v8<T>*>(p);
+__device__ __forceinline__ v8<T> load8_raw(const T* p, uint32_t left) {
+	if (left >= 8) return *reinterpret_cast<const v8<T>*>(p);
 	v8<T> x;
 #pragma unroll
 	for (int k = 0; k < 8; ++k) x[k] = (uint32_t)k < left ? p[k] : narrow<T>(0.0f);
 	return x;
 }
 template <class T>
-__device__ __forceinline__ void load8(const T* p, uint32_t left, bool wide, float (&v)[8]) {
-	const v8<T> x = load8_raw(p, left, wide);
+__device__ __forceinline__ void load8(const T* p, uint32_t left, float (&v)[8]) {
+	const v8<T> x = load8_raw(p, left);
 #pragma unroll
 	for (int k = 0; k < 8; ++k) v[k] = widen(x[k]);
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, uint32_t left, bool wide, const float (&v)[8]) {
-	if (wide && left >= 8) {
-		v8<T> x;
+__device__ __forceinline__ void store8(T* p, uint32_t left, const float (&v)[8]) {
+	v8<T> x;
 #pragma unroll
-		for (int k = 0; k < 8; ++k) x[k] = narrow<T>(v[k]);
+	for (int k = 0; k < 8; ++k) x[k] = narrow<T>(v[k]);
+	if (left >= 8) {
 		*reinterpret_cast<v8<T>*>(p) = x;
 	} else {
 #pragma unroll
 		for (int k = 0; k < 8; ++k)
-			if ((uint32_t)k < left) p[k] = narrow<T>(v[k]);
+			if ((uint32_t)k < left) p[k] = x[k];
 	}
 }
 
@@ -151,7 +151,8 @@ __device__ __forceinline__ float checkpoint_value(int q, uint32_t scale) {
 
 // Eight neighbouring values of one block (the first at a multiple of 8) to and from a checkpoint's row.  Adding 1.5 2^23
 // rounds to the nearest integer, ties to even, and leaves it in the sum's low bits.
-__device__ __forceinline__ void checkpoint_store8(int8_t* q, uint32_t left, bool wide, uint32_t scale, const float (&v)[8]) {
+typedef uint32_t q8 __attribute__((ext_vector_type(2), aligned(1)));
+__device__ __forceinline__ void checkpoint_store8(int8_t* q, uint32_t left, uint32_t scale, const float (&v)[8]) {
 	const int power = 133 - (int)scale;
 	uint32_t w[2];
 #pragma unroll
@@ -164,23 +165,23 @@ __device__ __forceinline__ void checkpoint_store8(int8_t* q, uint32_t left, bool
 		const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
 		w[h] = scale == 255u ? 0u : lo | hi;
 	}
-	if (wide && left >= 8) {
-		*reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+	if (left >= 8) {
+		*reinterpret_cast<q8*>(q) = q8{w[0], w[1]};
 	} else {
 #pragma unroll
 		for (int k = 0; k < 8; ++k)
 			if ((uint32_t)k < left) q[k] = (int8_t)(w[k / 4] >> (8 * (k % 4)));
 	}
 }
-__device__ __forceinline__ uint2 checkpoint_load8_raw(const int8_t* q, uint32_t left, bool wide) {
-	if (wide && left >= 8) return *reinterpret_cast<const uint2*>(q);
+__device__ __forceinline__ q8 checkpoint_load8_raw(const int8_t* q, uint32_t left) {
+	if (left >= 8) return *reinterpret_cast<const q8*>(q);
 	uint32_t w[2] = {0, 0};
 #pragma unroll
 	for (int k = 0; k < 8; ++k)
 		if ((uint32_t)k < left) w[k / 4] |= (uint32_t)(uint8_t)q[k] << (8 * (k % 4));
-	return make_uint2(w[0], w[1]);
+	return q8{w[0], w[1]};
 }
-__device__ __forceinline__ void checkpoint_widen8(uint2 w, uint32_t scale, float (&v)[8]) {
+__device__ __forceinline__ void checkpoint_widen8(q8 w, uint32_t scale, float (&v)[8]) {
 #pragma unroll
 	for (int k = 0; k < 8; ++k) v[k] = checkpoint_value((int8_t)((k < 4 ? w.x : w.y) >> (8 * (k % 4))), scale);
 }
@@ -199,18 +200,17 @@ struct Kept {
 	const int8_t* q = nullptr;
 	const uint8_t* scale = nullptr;
 	size_t q_stride = 0, scale_stride = 0;
-	bool wide = false;  // rows start on 16 bytes (a checkpoint's: on 8)
 	struct Raw {  // eight neighbouring values as they lie: of T, or eight q and their scale
 		v8<T> v;
-		uint2 q;
+		q8 q;
 		uint32_t scale;
 	};
 	__device__ __forceinline__ Raw raw8(size_t i, uint32_t j, uint32_t left) const {
 		Raw r = {};
 		if (v) {
-			r.v = load8_raw(v + i * stride + j, left, wide);
+			r.v = load8_raw(v + i * stride + j, left);
 		} else {
-			r.q = checkpoint_load8_raw(q + i * q_stride + j, left, wide);
+			r.q = checkpoint_load8_raw(q + i * q_stride + j, left);
 			r.scale = scale[i * scale_stride + (j >> 5)];
 		}
 		return r;
@@ -226,14 +226,14 @@ struct Kept {
 	__device__ __forceinline__ void at8(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const { widen8(raw8(i, j, left), x); }
 };
 
-inline bool wide_rows(const void* p, size_t stride, size_t element, size_t bytes = 16) {
-	return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * element % bytes == 0;
-}
-
 template <class T>
 inline Kept<T> kept(const void* v, uint32_t stride, const ngp_checkpoint8& c) {
-	return Kept<T>{static_cast<const T*>(v), stride, c.q, c.scale, c.q_stride, c.scale_stride,
-	               v ? wide_rows(v, stride, sizeof(T)) : wide_rows(c.q, c.q_stride, 1, 8)};
+	return Kept<T>{static_cast<const T*>(v), stride, c.q, c.scale, c.q_stride, c.scale_stride};
 }
+
+// out0[j] = the sum of part[0 .. shares)[j] for j < width, out1[j - width] the same of the next `width` columns if there are
+// any (columns = width or 2 width); either may be null.  In a fixed order.  (layer_norm.hip)
+void launch_column_sums(const float* part, uint32_t shares, uint32_t columns, uint32_t width, float* out0, float* out1,
+                        bool accumulate, hipStream_t s);
 
 }  // namespace ngp

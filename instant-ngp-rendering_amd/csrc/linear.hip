@@ -39,7 +39,6 @@ struct ForwardOut {
 	ngp_checkpoint8 z8;
 	size_t residual_stride, y_stride, z_stride;
 	int act;
-	bool residual_wide, y_wide, z_wide, z8_wide;
 	struct Columns {
 		float bias[8];
 	};
@@ -54,20 +53,20 @@ struct ForwardOut {
 	}
 	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
 		Fetched f = {};
-		if (residual) f.r = load8_raw(residual + i * residual_stride + j, left, residual_wide);
+		if (residual) f.r = load8_raw(residual + i * residual_stride + j, left);
 		return f;
 	}
 	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns& c, const Fetched& f, float (&v)[8],
 	                                       float (&kept)[8]) const {
 #pragma unroll
 		for (int k = 0; k < 8; ++k) kept[k] = v[k] += c.bias[k];
-		if (z) store8(z + i * z_stride + j, left, z_wide, v);
+		if (z) store8(z + i * z_stride + j, left, v);
 		act_values(act, v);
 		if (residual) {
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] += widen(f.r[k]);
 		}
-		store8(y + i * y_stride + j, left, y_wide, v);
+		store8(y + i * y_stride + j, left, v);
 	}
 };
 
@@ -77,9 +76,7 @@ struct GradientOut {  // dx
 	size_t stride;
 	Kept<T> p;
 	int act;
-	bool wide;
 	static constexpr ngp_checkpoint8 z8 = {};
-	static constexpr bool z8_wide = false;
 	struct Columns {};
 	typedef typename Kept<T>::Raw Fetched;
 	__device__ __forceinline__ Columns columns(uint32_t, uint32_t) const { return {}; }
@@ -95,7 +92,7 @@ struct GradientOut {  // dx
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] *= s[k];
 		}
-		store8(dx + i * stride + j, left, wide, v);
+		store8(dx + i * stride + j, left, v);
 	}
 };
 
@@ -103,9 +100,8 @@ template <class T>
 struct WeightsOut {  // dW
 	void* dw;
 	size_t stride;
-	bool f32, accumulate, wide;
+	bool f32, accumulate;
 	static constexpr ngp_checkpoint8 z8 = {};
-	static constexpr bool z8_wide = false;
 	struct Columns {};
 	struct Fetched {
 		float before[8];
@@ -113,7 +109,7 @@ struct WeightsOut {  // dW
 	__device__ __forceinline__ Columns columns(uint32_t, uint32_t) const { return {}; }
 	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
 		Fetched f = {};
-		if (accumulate) load8(static_cast<const float*>(dw) + i * stride + j, left, wide, f.before);
+		if (accumulate) load8(static_cast<const float*>(dw) + i * stride + j, left, f.before);
 		return f;
 	}
 	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns&, const Fetched& f, float (&v)[8],
@@ -121,9 +117,9 @@ struct WeightsOut {  // dW
 		if (f32) {
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] += f.before[k];
-			store8(static_cast<float*>(dw) + i * stride + j, left, wide, v);
+			store8(static_cast<float*>(dw) + i * stride + j, left, v);
 		} else {
-			store8(static_cast<T*>(dw) + i * stride + j, left, wide, v);
+			store8(static_cast<T*>(dw) + i * stride + j, left, v);
 		}
 	}
 };
@@ -280,7 +276,7 @@ __device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t 
 	top = quad_max(top);
 	if (!left) return;
 	const uint32_t scale = checkpoint_scale<T>(top);
-	checkpoint_store8(out.z8.q + i * out.z8.q_stride + j, left, out.z8_wide, scale, z);
+	checkpoint_store8(out.z8.q + i * out.z8.q_stride + j, left, scale, z);
 	if (j % 32u == 0) out.z8.scale[i * out.z8.scale_stride + j / 32u] = (uint8_t)scale;
 }
 
@@ -347,7 +343,7 @@ __device__ __forceinline__ void write_out(const ProductArgs& a, const Out& out, 
 			for (int u = 0; u < AHEAD; ++u) {
 				const size_t i = im + r0 + u * ROWS;
 				if (a.splits == 1) finish_block<T>(out, i, j, left[u], columns, fetched[u], v[u]);
-				else if (left[u]) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, true, v[u]);
+				else if (left[u]) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, v[u]);
 			}
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -528,7 +524,7 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 	if (in)
 		for (uint32_t s = 0; s < splits; ++s) {
 			float x[8];
-			load8(partial + ((size_t)s * M + i) * n8 + j, 8, true, x);
+			load8(partial + ((size_t)s * M + i) * n8 + j, 8, x);
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] += x[k];
 		}
@@ -551,7 +547,7 @@ __global__ void __launch_bounds__(256) k_lay_out(Kept<T> v, int act, size_t rows
 		act_values(act, x);
 #pragma unroll
 		for (int k = 0; k < 8; ++k) x[k] = j + k < width ? x[k] : 0.0f;
-		store8(to + t * 8u, 8, true, x);
+		store8(to + t * 8u, 8, x);
 	}
 }
 
@@ -575,7 +571,7 @@ __global__ void __launch_bounds__(256) k_linear_dz(Kept<T> dy, Kept<T> z, int ac
 #pragma unroll
 				for (int k = 0; k < 8; ++k) d[k] = j + k < width ? d[k] * s[k] : 0.0f;
 			}
-			if (dz) store8(dz + i * w8 + j, 8, true, d);
+			if (dz) store8(dz + i * w8 + j, 8, d);
 #pragma unroll
 			for (int k = 0; k < 8; ++k) sum[k] += d[k];
 		}
@@ -590,20 +586,6 @@ __global__ void __launch_bounds__(256) k_linear_dz(Kept<T> dy, Kept<T> z, int ac
 	float total = 0.0f;
 	for (uint32_t l = 0; l < lines; ++l) total += s[l * groups + threadIdx.x / 8u][threadIdx.x % 8u];
 	part[(size_t)blockIdx.y * width + column] = total;
-}
-
-__global__ void __launch_bounds__(256) k_column_sum(const float* __restrict__ part, uint32_t shares, uint32_t width, float* out,
-                                                    int accumulate) {
-	const uint32_t c = threadIdx.x % 16u, line = threadIdx.x / 16u, j = blockIdx.x * 16u + c;
-	float sum = 0.0f;
-	if (j < width)
-		for (uint32_t k = line; k < shares; k += 16u) sum += part[(size_t)k * width + j];
-	__shared__ float s[16][17];
-	s[line][c] = sum;
-	__syncthreads();
-	if (line || j >= width) return;
-	for (int l = 1; l < 16; ++l) sum += s[l][c];
-	out[j] = accumulate ? out[j] + sum : sum;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -673,10 +655,15 @@ static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size
 	}
 }
 
+// Whether a product's loads, 16 bytes at a time, can take a matrix where it lies.
+static bool in_place(const void* p, size_t stride, uint32_t width) {
+	return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && width % 8 == 0;
+}
+
 // `v` where it lies if the product can read it there, else act(v) copied to the workspace.
 template <class T>
 static Matrix operand(const Kept<T>& v, int act, size_t rows, uint32_t width, Room& room, hipStream_t s) {
-	if (v.v && v.wide && act == NGP_ACT_NONE && width % 8 == 0) return {v.v, v.stride};
+	if (v.v && act == NGP_ACT_NONE && in_place(v.v, v.stride, width)) return {v.v, v.stride};
 	T* to = room.take<T>(rows * up8(width));
 	if (room.run && rows) {
 		const size_t blocks = (rows * (up8(width) / 8) + 255) / 256;
@@ -693,9 +680,7 @@ static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) 
 	const Matrix x = operand<T>(kept<T>(a.x, a.x_stride, {}), NGP_ACT_NONE, a.n, a.n_in, room, s);
 	const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
 	const ForwardOut<T> out{a.bias, static_cast<const T*>(a.residual), static_cast<T*>(a.y), static_cast<T*>(a.z), a.z8,
-	                        a.residual_stride, a.y_stride, a.z_stride, a.activation,
-	                        wide_rows(a.residual, a.residual_stride, 2), wide_rows(a.y, a.y_stride, 2), wide_rows(a.z, a.z_stride, 2),
-	                        wide_rows(a.z8.q, a.z8.q_stride, 1, 8)};
+	                        a.residual_stride, a.y_stride, a.z_stride, a.activation};
 	product<T, ForwardOut<T>, false, false>(x, w, a.n, a.n_out, a.n_in, out, room, s);
 	return room.bytes;
 }
@@ -706,7 +691,7 @@ static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipSt
 	const bool products = a.dx || a.dweights, active = a.activation != NGP_ACT_NONE;
 	const Kept<T> dy = kept<T>(a.dy, a.dy_stride, {}), x = kept<T>(a.x, a.x_stride, a.x8);
 	// dz where it has to be made, or copied into rows that the products can read
-	const bool make_dz = products && (active || !dy.wide || a.n_out % 8);
+	const bool make_dz = products && (active || !in_place(a.dy, a.dy_stride, a.n_out));
 	T* dz_to = make_dz ? room.take<T>((size_t)a.n * up8(a.n_out)) : nullptr;
 	const Matrix dz = make_dz ? Matrix{dz_to, up8(a.n_out)} : Matrix{a.dy, a.dy_stride};
 	if (make_dz || a.dbias) {
@@ -721,21 +706,18 @@ static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipSt
 			k_linear_dz<T><<<dim3(wide, shares), 256, 0, s>>>(dy, kept<T>(a.z, a.z_stride, a.z8), a.activation, a.n, a.n_out, groups, each,
 			                                                 dz_to, part);
 			NGP_HIP_CHECK(hipGetLastError());
-			if (a.dbias) {
-				k_column_sum<<<(a.n_out + 15) / 16, 256, 0, s>>>(part, shares, a.n_out, a.dbias, a.accumulate);
-				NGP_HIP_CHECK(hipGetLastError());
-			}
+			if (a.dbias) launch_column_sums(part, shares, a.n_out, a.n_out, a.dbias, nullptr, a.accumulate != 0, s);
 		}
 	}
 	if (a.dx && a.n) {
 		const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
-		const GradientOut<T> out{static_cast<T*>(a.dx), a.dx_stride, x, a.x_activation, wide_rows(a.dx, a.dx_stride, 2)};
+		const GradientOut<T> out{static_cast<T*>(a.dx), a.dx_stride, x, a.x_activation};
 		product<T, GradientOut<T>, false, true>(dz, w, a.n, a.n_in, a.n_out, out, room, s);
 	}
 	if (a.dweights) {
 		const Matrix xs = operand<T>(x, a.x_activation, a.n, a.n_in, room, s);
 		const bool f32 = a.dweights_type == NGP_TYPE_F32;
-		const WeightsOut<T> out{a.dweights, a.dweights_stride, f32, a.accumulate != 0, wide_rows(a.dweights, a.dweights_stride, f32 ? 4 : 2)};
+		const WeightsOut<T> out{a.dweights, a.dweights_stride, f32, a.accumulate != 0};
 		product<T, WeightsOut<T>, true, true>(dz, xs, a.n_out, a.n_in, a.n, out, room, s);
 	}
 	return room.bytes;
