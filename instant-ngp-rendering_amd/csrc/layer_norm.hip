@@ -246,26 +246,33 @@ __global__ void __launch_bounds__(256) k_norm_backward_columns(ngp_layer_norm_ba
 	}
 }
 
-// 16 columns by 16 shares at a time.
-__global__ void __launch_bounds__(256) k_column_sums(const float* __restrict__ part, uint32_t shares, uint32_t columns, uint32_t width,
-                                                     float* out0, float* out1, bool accumulate) {
+// 16 columns by 64 shares at a time, four reads on their way; a wave's four shares meet by lane exchange, the 16 waves in LDS.
+__global__ void __launch_bounds__(1024) k_column_sums(const float* __restrict__ part, uint32_t shares, uint32_t columns, uint32_t width,
+                                                      float* out0, float* out1, bool accumulate) {
 	const uint32_t c = threadIdx.x % 16u, line = threadIdx.x / 16u, j = blockIdx.x * 16u + c;
-	float sum = 0.0f;
+	float sum[4] = {};
 	if (j < columns)
-		for (uint32_t k = line; k < shares; k += 16u) sum += part[(size_t)k * columns + j];
-	__shared__ float s[16][17];
-	s[line][c] = sum;
+		for (uint32_t k = line; k < shares; k += 256u)
+#pragma unroll
+			for (uint32_t u = 0; u < 4; ++u)
+				if (k + 64u * u < shares) sum[u] += part[(size_t)(k + 64u * u) * columns + j];
+	float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+	v += __shfl_xor(v, 16);
+	v += __shfl_xor(v, 32);
+	__shared__ float s[16][16];
+	if (threadIdx.x % 64u < 16u) s[threadIdx.x / 64u][c] = v;
 	__syncthreads();
 	if (line || j >= columns) return;
-	for (int l = 1; l < 16; ++l) sum += s[l][c];
+	v = 0.0f;
+	for (int w = 0; w < 16; ++w) v += s[w][c];
 	float* out = j < width ? out0 : out1;
 	const uint32_t o = j < width ? j : j - width;
-	if (out) out[o] = accumulate ? out[o] + sum : sum;
+	if (out) out[o] = accumulate ? out[o] + v : v;
 }
 
 void launch_column_sums(const float* part, uint32_t shares, uint32_t columns, uint32_t width, float* out0, float* out1, bool accumulate,
                         hipStream_t s) {
-	k_column_sums<<<(columns + 15) / 16, 256, 0, s>>>(part, shares, columns, width, out0, out1, accumulate);
+	k_column_sums<<<(columns + 15) / 16, 1024, 0, s>>>(part, shares, columns, width, out0, out1, accumulate);
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
@@ -302,7 +309,7 @@ struct NormBackwardPlan {
 	uint32_t grid, parts;
 };
 static NormBackwardPlan backward_plan(const ngp_layer_norm_backward_args& a) {
-	NormBackwardPlan p{norm_shape(a.n, a.width, 4), a.dgamma || a.dbeta, a.width <= NORM_IN_PASS, 0, 0};
+	NormBackwardPlan p{norm_shape(a.n, a.width, 2), a.dgamma || a.dbeta, a.width <= NORM_IN_PASS, 0, 0};
 	while (p.in_pass && p.shape.G > NORM_THREADS) p.shape.G /= 2, p.shape.chunks *= 2;
 	const uint32_t rows = NORM_THREADS / std::min(p.shape.G, NORM_THREADS);
 	p.grid = std::max(1u, std::min((a.n + rows - 1) / rows, 512u));
