@@ -430,11 +430,12 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, O
 }
 
 // 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
-// reads its next fragments and asks for a stage of K three ahead, and then they change places.  A barrier after each half
-// keeps the two sets of four waves in opposite phases; K goes in stages of 32 through four LDS buffers.
-template <class T, class Out, bool P_BY_K, bool Q_BY_K>
+// reads its next fragments and asks for a stage of K ahead, and then they change places.  A barrier after each half keeps
+// the two sets of four waves in opposite phases.  K goes through 128 KiB of LDS in stages of DEEP, each multiplied in steps
+// of 32: two buffers of 64 or four of 32.
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int DEEP>
 __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a, Out out) {
-	constexpr int BM = 256, BN = 256, TM = 4, TN = 2, DEEP = 32, BUFFERS = 4;
+	constexpr int BM = 256, BN = 256, TM = 4, TN = 2, BUFFERS = 128 / DEEP;
 	typedef Stage<T, BM, P_BY_K, DEEP, WIDE_THREADS> PStage;
 	typedef Stage<T, BN, Q_BY_K, DEEP, WIDE_THREADS> QStage;
 	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
@@ -469,42 +470,46 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 			__builtin_amdgcn_sched_barrier(0);
 			asm volatile("" ::: "memory");
 		};
-		// s_waitcnt with vmcnt = a wave's loads of two stages: all but the two latest stages it asked for are there; and
-		// lgkmcnt = 0: its reads are done
-		constexpr int WAIT = 2 * LOADS | 7 << 4;
-		static_assert(2 * LOADS < 16, "vmcnt's low field");
+		// s_waitcnt with lgkmcnt = 0, this wave's reads are done, and with vmcnt either 63, any loads may be on their way, or
+		// such that all but the latest BUFFERS - 2 stages it asked for are there
+		constexpr int READ = 15 | 7 << 4 | 3 << 14, ARRIVED = (BUFFERS - 2) * LOADS | 7 << 4;
+		static_assert((BUFFERS - 2) * LOADS < 16, "vmcnt's low field");
 		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % DEEP) + 1u;
 		ps.load_first(lds, k_in);
 		qs.load_first(lds + PStage::BYTES, k_in);
-		load(1);
-		load(2);
-		__builtin_amdgcn_s_waitcnt(WAIT);
+#pragma unroll
+		for (int s = 1; s < BUFFERS - 1; ++s) load(s);
+		__builtin_amdgcn_s_waitcnt(ARRIVED);
 		meet();
-		if (wave >= 4u) meet();  // the second set runs half a stage behind
+		if (wave >= 4u) meet();  // the second set runs half a step behind
 		for (uint32_t s = 0; s < stages; ++s) {
 			// the buffer of stage s - 1 is free: both sets have read it, the second before the barrier just passed
-			load(s + 3);
+			load(s + BUFFERS - 1);
 			const char* from = lds + s % BUFFERS * STAGE;
-			s16x8 p[2][TM], q[2][TN];
 #pragma unroll
-			for (int k = 0; k < 2; ++k) {
+			for (int step = 0; step < DEEP / 32; ++step) {
+				s16x8 p[2][TM], q[2][TN];
 #pragma unroll
-				for (int t = 0; t < TN; ++t) q[k][t] = qf.read(from + PStage::BYTES, k, t);
+				for (int k = 0; k < 2; ++k) {
 #pragma unroll
-				for (int t = 0; t < TM; ++t) p[k][t] = pf.read(from, k, t);
+					for (int t = 0; t < TN; ++t) q[k][t] = qf.read(from + PStage::BYTES, 2 * step + k, t);
+#pragma unroll
+					for (int t = 0; t < TM; ++t) p[k][t] = pf.read(from, 2 * step + k, t);
+				}
+				// before the next stage is read: it has arrived as far as this wave asked for it; the barriers tell of the others
+				if (step == DEEP / 32 - 1) __builtin_amdgcn_s_waitcnt(ARRIVED);
+				else __builtin_amdgcn_s_waitcnt(READ);
+				meet();
+				__builtin_amdgcn_s_setprio(1);
+#pragma unroll
+				for (int k = 0; k < 2; ++k)
+#pragma unroll
+					for (int n = 0; n < TN; ++n)
+#pragma unroll
+						for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k][n], p[k][m], c[n][m]);
+				__builtin_amdgcn_s_setprio(0);
+				meet();
 			}
-			// stage s + 1 has arrived as far as this wave asked for it; the barriers up to its reading tell of the others
-			__builtin_amdgcn_s_waitcnt(WAIT);
-			meet();
-			__builtin_amdgcn_s_setprio(1);
-#pragma unroll
-			for (int k = 0; k < 2; ++k)
-#pragma unroll
-				for (int n = 0; n < TN; ++n)
-#pragma unroll
-					for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k][n], p[k][m], c[n][m]);
-			__builtin_amdgcn_s_setprio(0);
-			meet();
 		}
 		if (wave < 4u) meet();
 		__builtin_amdgcn_s_waitcnt(0);
@@ -645,7 +650,7 @@ static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size
 	ProductArgs a{p, q, M, K, plan.k_each, N, plan.tiles_m, plan.tiles_n, plan.splits, nullptr};
 	if (plan.splits > 1) a.partial = room.take<float>((size_t)plan.splits * M * up8(N));
 	if (!room.run) return;
-	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K>, WIDE_THREADS, 131072, a, out, s);
+	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, WIDE_THREADS, 131072, a, out, s);
 	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128>, PRODUCT_THREADS, 65536, a, out, s);
 	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64>, PRODUCT_THREADS, 32768, a, out, s);
 	if (plan.splits > 1) {
