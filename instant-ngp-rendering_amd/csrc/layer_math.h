@@ -209,27 +209,35 @@ struct Kept {
 	const int8_t* q = nullptr;
 	const uint8_t* scale = nullptr;
 	size_t q_stride = 0, scale_stride = 0;
-	struct Raw {  // eight neighbouring values as they lie: of T, or eight q and their scale
-		v8<T> v;
-		q8 q;
+	struct Raw {  // eight neighbouring values as they lie: of T, or eight q in the first words and their scale
+		uint32_t w[sizeof(T) * 2];
 		uint32_t scale;
 	};
-	__device__ __forceinline__ Raw raw8(size_t i, uint32_t j, uint32_t left) const {
+	__device__ __forceinline__ Raw raw8_values(size_t i, uint32_t j, uint32_t left) const {
 		Raw r = {};
-		if (v) {
-			r.v = load8_raw(v + i * stride + j, left);
-		} else {
-			r.q = checkpoint_load8_raw(q + i * q_stride + j, left);
-			r.scale = scale[i * scale_stride + (j >> 5)];
-		}
+		const v8<T> x = load8_raw(v + i * stride + j, left);
+		__builtin_memcpy(r.w, &x, sizeof(r.w));
 		return r;
+	}
+	__device__ __forceinline__ Raw raw8_checkpoint(size_t i, uint32_t j, uint32_t left) const {
+		Raw r = {};
+		const q8 x = checkpoint_load8_raw(q + i * q_stride + j, left);
+		r.w[0] = x[0];
+		r.w[1] = x[1];
+		r.scale = scale[i * scale_stride + (j >> 5)];
+		return r;
+	}
+	__device__ __forceinline__ Raw raw8(size_t i, uint32_t j, uint32_t left) const {
+		return v ? raw8_values(i, j, left) : raw8_checkpoint(i, j, left);
 	}
 	__device__ __forceinline__ void widen8(const Raw& r, float (&x)[8]) const {
 		if (v) {
+			v8<T> y;
+			__builtin_memcpy(&y, r.w, sizeof(r.w));
 #pragma unroll
-			for (int k = 0; k < 8; ++k) x[k] = widen(r.v[k]);
+			for (int k = 0; k < 8; ++k) x[k] = widen(y[k]);
 		} else {
-			checkpoint_widen8(r.q, r.scale, x);
+			checkpoint_widen8(q8{r.w[0], r.w[1]}, r.scale, x);
 		}
 	}
 	__device__ __forceinline__ void at8(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const { widen8(raw8(i, j, left), x); }

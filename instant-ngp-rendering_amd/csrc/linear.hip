@@ -29,7 +29,10 @@ __device__ __forceinline__ f32x16 mfma(bf16, s16x8 a, s16x8 b, f32x16 c) {
 }
 
 // ---- what a product does with its fp32 sums, eight neighbouring columns of a row at a time --------------------------
-// Columns: what the rows share; Fetched: what is read for a row's eight, asked for before any of them is finished.
+// Columns: what the rows share; Fetched: what is read for a row's eight, asked for before any of them is finished, by a
+// `fetch` for each kind of source (by_kind), so that no branch stands among the loads and they wait for nothing.
+template <int K>
+using Kind = std::integral_constant<int, K>;
 template <class T>
 struct ForwardOut {
 	const float* bias;
@@ -42,19 +45,19 @@ struct ForwardOut {
 	struct Columns {
 		float bias[8];
 	};
-	struct Fetched {
-		v8<T> r;
-	};
+	typedef v8<T> Fetched;
 	__device__ __forceinline__ Columns columns(uint32_t j, uint32_t left) const {
 		Columns c;
 #pragma unroll
 		for (int k = 0; k < 8; ++k) c.bias[k] = bias && (uint32_t)k < left ? bias[j + k] : 0.0f;
 		return c;
 	}
-	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
-		Fetched f = {};
-		if (residual) f.r = load8_raw(residual + i * residual_stride + j, left);
-		return f;
+	template <class F>
+	__device__ __forceinline__ void by_kind(F f) const { residual ? f(Kind<1>{}) : f(Kind<0>{}); }
+	template <int K>
+	__device__ __forceinline__ Fetched fetch(Kind<K>, size_t i, uint32_t j, uint32_t left) const {
+		if constexpr (K == 1) return load8_raw(residual + i * residual_stride + j, left);
+		else return {};
 	}
 	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns& c, const Fetched& f, float (&v)[8],
 	                                       float (&kept)[8]) const {
@@ -64,7 +67,7 @@ struct ForwardOut {
 		act_values(act, v);
 		if (residual) {
 #pragma unroll
-			for (int k = 0; k < 8; ++k) v[k] += widen(f.r[k]);
+			for (int k = 0; k < 8; ++k) v[k] += widen(f[k]);
 		}
 		store8(y + i * y_stride + j, left, v);
 	}
@@ -80,8 +83,13 @@ struct GradientOut {  // dx
 	struct Columns {};
 	typedef typename Kept<T>::Raw Fetched;
 	__device__ __forceinline__ Columns columns(uint32_t, uint32_t) const { return {}; }
-	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
-		return act == NGP_ACT_NONE ? Fetched{} : p.raw8(i, j, left);
+	template <class F>
+	__device__ __forceinline__ void by_kind(F f) const { act == NGP_ACT_NONE ? f(Kind<0>{}) : p.v ? f(Kind<1>{}) : f(Kind<2>{}); }
+	template <int K>
+	__device__ __forceinline__ Fetched fetch(Kind<K>, size_t i, uint32_t j, uint32_t left) const {
+		if constexpr (K == 1) return p.raw8_values(i, j, left);
+		else if constexpr (K == 2) return p.raw8_checkpoint(i, j, left);
+		else return {};
 	}
 	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns&, const Fetched& f, float (&v)[8],
 	                                       float (&)[8]) const {
@@ -107,9 +115,12 @@ struct WeightsOut {  // dW
 		float before[8];
 	};
 	__device__ __forceinline__ Columns columns(uint32_t, uint32_t) const { return {}; }
-	__device__ __forceinline__ Fetched fetch(size_t i, uint32_t j, uint32_t left) const {
+	template <class F>
+	__device__ __forceinline__ void by_kind(F f) const { accumulate ? f(Kind<1>{}) : f(Kind<0>{}); }
+	template <int K>
+	__device__ __forceinline__ Fetched fetch(Kind<K>, size_t i, uint32_t j, uint32_t left) const {
 		Fetched f = {};
-		if (accumulate) load8(static_cast<const float*>(dw) + i * stride + j, left, f.before);
+		if constexpr (K == 1) load8(static_cast<const float*>(dw) + i * stride + j, left, f.before);
 		return f;
 	}
 	__device__ __forceinline__ void finish(size_t i, uint32_t j, uint32_t left, const Columns&, const Fetched& f, float (&v)[8],
@@ -272,7 +283,7 @@ __device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t 
 	if (!out.z8.q) return;
 	uint32_t top = 0;
 #pragma unroll
-	for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left ? magnitude_bits(z[k]) : 0u);
+	for (int k = 0; k < 8; ++k) top = max(top, magnitude_bits(z[k]));  // past the row's end: 0 (Q's rows are), or as the row
 	top = quad_max(top);
 	if (!left) return;
 	const uint32_t scale = checkpoint_scale<T>(top);
@@ -306,49 +317,79 @@ struct Place {
 // one copy of the code that finishes a value.
 template <int TN>
 constexpr int STRIP = 32 * (TN * 32 + 4);  // floats; + 4: 32 rows' 16-byte pieces on different banks
+// What the caller's matrices hold for a strip is asked for a strip ahead, for the first one before K is gone through.
 template <class T, class Out, int TM, int TN>
-__device__ __forceinline__ void write_out(const ProductArgs& a, const Out& out, uint32_t split, size_t i0, uint32_t j0, float* strip,
-                                          const f32x16 (&c)[TN][TM]) {
-	constexpr int PITCH = TN * 32 + 4, LANES = TN * 4;
-	const uint32_t lane = threadIdx.x & 63u, n8 = (a.N + 7u) & ~7u, j = j0 + lane % LANES * 8u;
-	const auto columns = out.columns(j, j < a.N ? a.N - j : 0u);
+struct WriteOut {
+	static constexpr int PITCH = TN * 32 + 4, LANES = TN * 4, ROWS = 64 / LANES, TURNS = 32 / ROWS;
+	const ProductArgs& a;
+	const Out& out;
+	size_t i0;      // the lane's first row,
+	uint32_t j;     // its columns,
+	uint32_t left;  // how many there are
+	bool whole;     // the wave's tiles lie inside C: nothing is looked at again
+	typename Out::Fetched ahead[TURNS];
+
+	__device__ __forceinline__ WriteOut(const ProductArgs& a, const Out& out, size_t i, uint32_t j0) : a(a), out(out) {
+		const uint32_t lane = threadIdx.x & 63u;
+		i0 = i + lane / LANES;
+		j = j0 + lane % LANES * 8u;
+		left = j < a.N ? a.N - j : 0u;
+		whole = i + TM * 32u <= a.M && j0 + TN * 32u <= a.N;
 #pragma unroll
-	for (int m = 0; m < TM; ++m) {
-#pragma unroll
-		for (int n = 0; n < TN; ++n)
-#pragma unroll
-			for (int g = 0; g < 4; ++g)
-				*reinterpret_cast<f32x4*>(strip + (lane & 31u) * PITCH + n * 32 + g * 8 + (lane >> 5) * 4u) =
-				    f32x4{c[n][m][4 * g], c[n][m][4 * g + 1], c[n][m][4 * g + 2], c[n][m][4 * g + 3]};
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-		// four rows' reads are on their way before the first of them is worked on: the wave has its SIMD to itself
-		constexpr int ROWS = 64 / LANES, AHEAD = 32 / ROWS < 4 ? 32 / ROWS : 4;
-#pragma unroll 1
-		for (uint32_t r0 = lane / LANES; r0 < 32u; r0 += ROWS * AHEAD) {
-			const size_t im = i0 + m * 32u;
-			float v[AHEAD][8];
-			typename Out::Fetched fetched[AHEAD];
-			uint32_t left[AHEAD];
-#pragma unroll
-			for (int u = 0; u < AHEAD; ++u) {
-				const uint32_t r = r0 + u * ROWS;
-				const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u);
-				const f32x4 hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + lane % LANES * 8u + 4);
-#pragma unroll
-				for (int k = 0; k < 8; ++k) v[u][k] = k < 4 ? lo[k & 3] : hi[k & 3];
-				left[u] = im + r < a.M && j < a.N ? a.N - j : 0u;
-				if (left[u] && a.splits == 1) fetched[u] = out.fetch(im + r, j, left[u]);
-			}
-#pragma unroll
-			for (int u = 0; u < AHEAD; ++u) {
-				const size_t i = im + r0 + u * ROWS;
-				if (a.splits == 1) finish_block<T>(out, i, j, left[u], columns, fetched[u], v[u]);
-				else if (left[u]) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, v[u]);
-			}
-		}
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		for (int u = 0; u < TURNS; ++u) ahead[u] = {};
+		if (a.splits == 1) whole ? fetch<true>(0) : fetch<false>(0);
 	}
-}
+	template <bool WHOLE>
+	__device__ __forceinline__ uint32_t here(int m, int u) const {
+		return WHOLE ? 8u : i0 + m * 32u + u * ROWS < a.M ? left : 0u;
+	}
+	template <bool WHOLE>
+	__device__ __forceinline__ void fetch(int m) {
+		out.by_kind([&](auto kind) {
+#pragma unroll
+			for (int u = 0; u < TURNS; ++u)
+				if (here<WHOLE>(m, u)) ahead[u] = out.fetch(kind, i0 + m * 32u + u * ROWS, j, here<WHOLE>(m, u));
+		});
+	}
+	template <bool WHOLE, bool JOIN>
+	__device__ __forceinline__ void write(uint32_t split, float* strip, const f32x16 (&c)[TN][TM]) {
+		const uint32_t lane = threadIdx.x & 63u, n8 = (a.N + 7u) & ~7u;
+		typename Out::Columns columns;
+		if constexpr (!JOIN) columns = out.columns(j, WHOLE ? 8u : left);
+#pragma unroll
+		for (int m = 0; m < TM; ++m) {
+			typename Out::Fetched fetched[TURNS];
+#pragma unroll
+			for (int u = 0; u < TURNS; ++u) fetched[u] = ahead[u];
+			if constexpr (!JOIN)
+				if (m + 1 < TM) fetch<WHOLE>(m + 1);
+#pragma unroll
+			for (int n = 0; n < TN; ++n)
+#pragma unroll
+				for (int g = 0; g < 4; ++g)
+					*reinterpret_cast<f32x4*>(strip + (lane & 31u) * PITCH + n * 32 + g * 8 + (lane >> 5) * 4u) =
+					    f32x4{c[n][m][4 * g], c[n][m][4 * g + 1], c[n][m][4 * g + 2], c[n][m][4 * g + 3]};
+			__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+			for (int u = 0; u < TURNS; ++u) {
+				const float* row = strip + (lane / LANES + u * ROWS) * PITCH + lane % LANES * 8u;
+				const f32x4 lo = *reinterpret_cast<const f32x4*>(row), hi = *reinterpret_cast<const f32x4*>(row + 4);
+				float v[8];
+#pragma unroll
+				for (int k = 0; k < 8; ++k) v[k] = k < 4 ? lo[k & 3] : hi[k & 3];
+				const size_t i = i0 + m * 32u + u * ROWS;
+				if constexpr (!JOIN) finish_block<T>(out, i, j, here<WHOLE>(m, u), columns, fetched[u], v);
+				else if (here<WHOLE>(m, u)) store8(a.partial + ((size_t)split * a.M + i) * n8 + j, 8, v);
+			}
+			__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		}
+	}
+	__device__ __forceinline__ void operator()(uint32_t split, float* strip, const f32x16 (&c)[TN][TM]) {
+		if (a.splits > 1) write<false, true>(split, strip, c);
+		else if (whole) write<true, false>(split, strip, c);
+		else write<false, false>(split, strip, c);
+	}
+};
 
 // BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through two LDS buffers: while the matrix cores
 // work on one stage, the next is on its way from memory into the other buffer without passing registers.  P's rows are
@@ -367,6 +408,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, O
 	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
 	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + 63u) / 64u);
 
+	WriteOut<T, Out, TM, TN> write_out(a, out, at.m0 + wm, at.n0 + wn);
 	f32x16 c[TN][TM] = {};
 	if (stages) {
 		PStage ps;
@@ -426,7 +468,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, O
 		__builtin_amdgcn_s_waitcnt(0);
 	}
 	__syncthreads();  // the last stage has been read
-	write_out<T, Out, TM, TN>(a, out, at.split, at.m0 + wm, at.n0 + wn, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
+	write_out(at.split, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
 }
 
 // 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
@@ -447,6 +489,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 	const uint32_t wm = wave / 4u * 128u, wn = wave % 4u * 64u;
 	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + DEEP - 1) / DEEP);
 
+	WriteOut<T, Out, TM, TN> write_out(a, out, at.m0 + wm, at.n0 + wn);
 	f32x16 c[TN][TM] = {};
 	if (stages) {
 		PStage ps;
@@ -515,7 +558,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 		__builtin_amdgcn_s_waitcnt(0);
 	}
 	__syncthreads();
-	write_out<T, Out, TM, TN>(a, out, at.split, at.m0 + wm, at.n0 + wn, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
+	write_out(at.split, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
 }
 
 // The splits' sums, in their order, to where the product would have put them.
@@ -535,7 +578,7 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 		}
 	const uint32_t left = in ? N - j : 0u;
 	typename Out::Fetched fetched = {};
-	if (left) fetched = out.fetch(i, j, left);
+	if (left) out.by_kind([&](auto kind) { fetched = out.fetch(kind, i, j, left); });
 	finish_block<T>(out, i, j, left, out.columns(j, left), fetched, v);
 }
 
