@@ -10,25 +10,6 @@
 
 namespace ngp {
 
-// Where a thread is among rows of `eighths` items, and how it steps by the whole grid without dividing again.
-struct Walk {
-	size_t i, di;
-	uint32_t e, de, eighths;
-	__device__ __forceinline__ explicit Walk(uint32_t eighths) : eighths(eighths) {
-		const size_t t = (size_t)blockIdx.x * 256u + threadIdx.x;
-		const uint32_t step = gridDim.x * 256u;
-		i = t / eighths;
-		e = (uint32_t)(t % eighths);
-		di = step / eighths;
-		de = step % eighths;
-	}
-	__device__ __forceinline__ void next() {
-		i += di;
-		e += de;
-		if (e >= eighths) e -= eighths, ++i;
-	}
-};
-
 // Four items per block of 32, of which the last ones of a row may have nothing to do; a quad leaves the loop together.
 template <class T>
 __global__ void __launch_bounds__(256) k_checkpoint_store(Kept<T> v, size_t n, uint32_t width, ngp_checkpoint8 c) {

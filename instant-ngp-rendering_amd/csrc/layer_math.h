@@ -201,6 +201,26 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 	return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
 }
 
+// Where a thread of a workgroup of 256 is among rows of `eighths` items, and how it steps by the whole grid without dividing
+// again.
+struct Walk {
+	size_t i, di;
+	uint32_t e, de, eighths;
+	__device__ __forceinline__ explicit Walk(uint32_t eighths) : eighths(eighths) {
+		const size_t t = (size_t)blockIdx.x * 256u + threadIdx.x;
+		const uint32_t step = gridDim.x * 256u;
+		i = t / eighths;
+		e = (uint32_t)(t % eighths);
+		di = step / eighths;
+		de = step % eighths;
+	}
+	__device__ __forceinline__ void next() {
+		i += di;
+		e += de;
+		if (e >= eighths) e -= eighths, ++i;
+	}
+};
+
 // Activations as a backward pass finds them: [rows][stride] of T, or a checkpoint (v null), or absent (both null).
 template <class T>
 struct Kept {
@@ -238,6 +258,15 @@ struct Kept {
 			for (int k = 0; k < 8; ++k) x[k] = widen(y[k]);
 		} else {
 			checkpoint_widen8(q8{r.w[0], r.w[1]}, r.scale, x);
+		}
+	}
+	template <bool VALUES>
+	__device__ __forceinline__ void at8_of(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const {
+		if constexpr (VALUES) {
+			load8(v + i * stride + j, left, x);
+		} else {
+			const q8 w = checkpoint_load8_raw(q + i * q_stride + j, left);
+			checkpoint_widen8(w, scale[i * scale_stride + (j >> 5)], x);
 		}
 	}
 	__device__ __forceinline__ void at8(size_t i, uint32_t j, uint32_t left, float (&x)[8]) const { widen8(raw8(i, j, left), x); }

@@ -584,18 +584,18 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 
 // ---- operands that do not lie as the product wants them ---------------------------------------------------------------
 // act(v), rounded to T, in rows of `width` up to 8, filled up with zeros.
-template <class T>
+template <class T, bool VALUES>
 __global__ void __launch_bounds__(256) k_lay_out(Kept<T> v, int act, size_t rows, uint32_t width, T* __restrict__ to) {
-	const uint32_t chunks = (width + 7u) / 8u;
-	for (size_t t = (size_t)blockIdx.x * 256u + threadIdx.x; t < rows * chunks; t += (size_t)gridDim.x * 256u) {
-		const size_t i = t / chunks;
-		const uint32_t j = (uint32_t)(t % chunks) * 8u;
+	const uint32_t w8 = (width + 7u) & ~7u;
+	for (Walk w(w8 / 8u); w.i < rows; w.next()) {
+		const uint32_t j = w.e * 8u;
 		float x[8];
-		v.at8(i, j, width - j, x);
+		v.template at8_of<VALUES>(w.i, j, width - j, x);
 		act_values(act, x);
+		if (width - j < 8u)
 #pragma unroll
-		for (int k = 0; k < 8; ++k) x[k] = j + k < width ? x[k] : 0.0f;
-		store8(to + t * 8u, 8, x);
+			for (int k = 0; k < 8; ++k) x[k] = j + k < width ? x[k] : 0.0f;
+		store8(to + w.i * w8 + j, 8, x);
 	}
 }
 
@@ -715,7 +715,8 @@ static Matrix operand(const Kept<T>& v, int act, size_t rows, uint32_t width, Ro
 	T* to = room.take<T>(rows * up8(width));
 	if (room.run && rows) {
 		const size_t blocks = (rows * (up8(width) / 8) + 255) / 256;
-		k_lay_out<T><<<(uint32_t)std::min<size_t>(blocks, 16384), 256, 0, s>>>(v, act, rows, width, to);
+		auto kernel = v.v ? k_lay_out<T, true> : k_lay_out<T, false>;
+		kernel<<<(uint32_t)std::min<size_t>(blocks, 16384), 256, 0, s>>>(v, act, rows, width, to);
 		NGP_HIP_CHECK(hipGetLastError());
 	}
 	return {to, up8(width)};
