@@ -250,12 +250,15 @@ struct Kept {
 	__device__ __forceinline__ Raw raw8(size_t i, uint32_t j, uint32_t left) const {
 		return v ? raw8_values(i, j, left) : raw8_checkpoint(i, j, left);
 	}
+	__device__ __forceinline__ void widen8_values(const Raw& r, float (&x)[8]) const {
+		v8<T> y;
+		__builtin_memcpy(&y, r.w, sizeof(r.w));
+#pragma unroll
+		for (int k = 0; k < 8; ++k) x[k] = widen(y[k]);
+	}
 	__device__ __forceinline__ void widen8(const Raw& r, float (&x)[8]) const {
 		if (v) {
-			v8<T> y;
-			__builtin_memcpy(&y, r.w, sizeof(r.w));
-#pragma unroll
-			for (int k = 0; k < 8; ++k) x[k] = widen(y[k]);
+			widen8_values(r, x);
 		} else {
 			checkpoint_widen8(q8{r.w[0], r.w[1]}, r.scale, x);
 		}

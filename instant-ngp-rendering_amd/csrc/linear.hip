@@ -28,6 +28,17 @@ __device__ __forceinline__ f32x16 mfma(bf16, s16x8 a, s16x8 b, f32x16 c) {
 	return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8<bf16>, a), __builtin_bit_cast(v8<bf16>, b), c, 0, 0, 0);
 }
 
+// Half h of a 32 x 32 tile's columns: register r holds column r % 4 + 8 (r / 4) + 4 (lane / 32) of row lane % 32; groups of
+// four columns change places between the half waves, which leaves a lane the eight at 16 h + 8 (lane / 32).
+__device__ __forceinline__ void eight(const f32x16& c, int h, float (&v)[8]) {
+#pragma unroll
+	for (int k = 0; k < 4; ++k) {
+		const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[8 * h + k]), __float_as_uint(c[8 * h + 4 + k]), false, false);
+		v[k] = __uint_as_float(s[0]);
+		v[k + 4] = __uint_as_float(s[1]);
+	}
+}
+
 // ---- what a product does with its fp32 sums, eight neighbouring columns of a row at a time --------------------------
 // Columns: what the rows share; Fetched: what is read for a row's eight, asked for before any of them is finished, by a
 // `fetch` for each kind of source (by_kind), so that no branch stands among the loads and they wait for nothing.
@@ -561,25 +572,225 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 	write_out(at.split, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
 }
 
-// The splits' sums, in their order, to where the product would have put them.
+// The splits' sums to where the product would have put them.  `lines` threads (a power of two up to 32) share an eight's
+// splits, each the ones in its turn; their sums meet in a fixed order.  Four neighbouring threads finish a block of 32.
 template <class T, class Out>
-__global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ partial, uint32_t splits, size_t M, uint32_t N, Out out) {
-	const uint32_t n8 = (N + 7u) & ~7u, chunks = (N + 31u) / 32u * 4u;  // four threads to a block of 32
-	const size_t t = (size_t)blockIdx.x * 256u + threadIdx.x, i = t / chunks;
+__global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ partial, uint32_t splits, size_t M, uint32_t N, uint32_t lines, Out out) {
+	const uint32_t n8 = (N + 7u) & ~7u, chunks = (N + 31u) / 32u * 4u, items = 256u / lines;
+	const uint32_t item = threadIdx.x % items, line = threadIdx.x / items;
+	const size_t t = (size_t)blockIdx.x * items + item, i = t / chunks;
 	const uint32_t j = (uint32_t)(t % chunks) * 8u;
 	const bool in = i < M && j < N;
 	float v[8] = {};
 	if (in)
-		for (uint32_t s = 0; s < splits; ++s) {
+		for (uint32_t s = line; s < splits; s += lines) {
 			float x[8];
 			load8(partial + ((size_t)s * M + i) * n8 + j, 8, x);
 #pragma unroll
 			for (int k = 0; k < 8; ++k) v[k] += x[k];
 		}
+	if (lines > 1) {
+		__shared__ float sums[8][256];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) sums[k][threadIdx.x] = v[k];
+		__syncthreads();
+		if (line) return;
+		for (uint32_t l = 1; l < lines; ++l)
+#pragma unroll
+			for (int k = 0; k < 8; ++k) v[k] += sums[k][l * items + item];
+	}
 	const uint32_t left = in ? N - j : 0u;
 	typename Out::Fetched fetched = {};
 	if (left) out.by_kind([&](auto kind) { fetched = out.fetch(kind, i, j, left); });
 	finish_block<T>(out, i, j, left, out.columns(j, left), fetched, v);
+}
+
+// ---- narrow layers ------------------------------------------------------------------------------------------------------
+// Backward of layers of up to 128 x 128 over many rows: memory bound, so all of it in one pass over dy, z and x.  Persistent
+// workgroups of four waves take ROWS rows at a time: dz and the layer's input go to LDS in 16 bits ([row][feature], from
+// where dx reads dz along its rows and dW reads both transposed), the weights' fragments and the workgroup's share of dW stay
+// in registers, the next rows are on their way from memory meanwhile.  dW and db leave as a share per workgroup.
+// 64 -> 64 over 2^18 rows moves 134 MB instead of the 233 MB of separate passes.
+template <class T>
+struct NarrowArgs {
+	Kept<T> dy, z, x;
+	int act, x_act;
+	const T* w;
+	size_t w_stride, n;
+	uint32_t n_in, n_out;
+	T* dx;
+	size_t dx_stride;
+	float *dw_part, *db_part;  // [workgroup][n_out][n_in up to 8], [workgroup][n_out]
+};
+
+template <class T, int NI, int NO, bool EVEN>
+__global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(NarrowArgs<T> a) {
+	constexpr int ROWS = NI + NO > 128 ? 64 : 128;
+	constexpr int DZ_ITEMS = ROWS * NO / 8 / 256, X_ITEMS = ROWS * NI / 8 / 256;  // eights per thread
+	constexpr int STRIPS = ROWS / 32, NT = NI / 32 / (4 / STRIPS);               // a wave's strip of dx: NT tiles of 32 columns
+	constexpr int MW = NO / 32, WT = MW * (NI / 32) / 4;                           // dW: rows of tiles, tiles per wave
+	__shared__ __attribute__((aligned(16))) char lds[ROWS * (NO + NI) * 2];
+	char* const lds_dz = lds;
+	char* const lds_x = lds + ROWS * NO * 2;
+	const uint32_t tid = threadIdx.x, wave = tid / 64u, lane = tid & 63u;
+	// 16-byte chunk c of a row lies at c ^ twist(row): 16 rows' same chunk (read along the rows) and 4 rows' 64 bytes (read
+	// transposed) are each on all banks once
+	auto twist = [](uint32_t r, int width) {
+		return width == 64 ? (r & 2u) << 1 | (r & 4u) >> 1 | (r & 8u) >> 3 : (r & 3u) << 2 | ((r >> 2) & 3u);
+	};
+	auto place = [&](uint32_t r, uint32_t c, int width) { return r * (width * 2) + ((c ^ twist(r, width)) << 4); };
+	// a transposed fragment's two halves: column tile t of rows 16 s ..
+	auto transposed = [&](const char* from, int width, int s, uint32_t t) {
+		typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+		const uint32_t g = lane >> 4, q = (lane & 15u) >> 2, p = lane & 3u, c = t * 4u + 2u * (g & 1u) + (p >> 1);
+		const uint32_t r = 8u * (g >> 1) + q;  // (the twist repeats every 16 rows)
+		from += s * 16 * (width * 2) + (p & 1u) * 8u;
+		const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(from + place(r, c, width)));
+		const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(from + place(r + 4u, c, width)));
+		return s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+	};
+
+	// the weights as dx's Q: row = input, k = output
+	const uint32_t strip = wave % STRIPS, nt0 = wave / STRIPS * NT;
+	s16x8 w[NT][NO / 16] = {};
+	if (a.dx)
+#pragma unroll
+		for (int t = 0; t < NT; ++t)
+#pragma unroll
+			for (int s = 0; s < NO / 16; ++s)
+#pragma unroll
+				for (int k = 0; k < 8; ++k) {
+					const uint32_t row = (nt0 + t) * 32u + (lane & 31u), out = s * 16u + 8u * (lane >> 5) + k;
+					if (row < a.n_in && out < a.n_out) w[t][s][k] = __builtin_bit_cast(short, a.w[out * a.w_stride + row]);
+				}
+
+	f32x16 dw[WT] = {};
+	float db[8] = {};
+	typename Kept<T>::Raw dy[DZ_ITEMS], z[DZ_ITEMS], x[X_ITEMS];
+	auto items = [&](size_t row0, auto kind, const Kept<T>& m, uint32_t width, int padded, auto& raw, auto count) {
+#pragma unroll
+		for (int k = 0; k < count; ++k) {
+			const uint32_t item = tid + k * 256u, c = item % (padded / 8u) * 8u;
+			const size_t i = row0 + item / (padded / 8u);
+			if constexpr (EVEN) {  // both widths are multiples of 8: rows and chunks that are not there are read as the last row's or the first chunk, and not used
+				const size_t ic = min(i, a.n - 1);
+				const uint32_t cc = c < width ? c : 0u;
+				raw[k] = kind == 1 ? m.raw8_values(ic, cc, 8) : m.raw8_checkpoint(ic, cc, 8);
+			} else {
+				raw[k] = {};
+				if (i < a.n && c < width) raw[k] = kind == 1 ? m.raw8_values(i, c, width - c) : m.raw8_checkpoint(i, c, width - c);
+			}
+		}
+	};
+	auto ask = [&](size_t row0) {
+		items(row0, Kind<1>{}, a.dy, a.n_out, NO, dy, Kind<DZ_ITEMS>{});
+		if (a.act != NGP_ACT_NONE) {
+			if (a.z.v) items(row0, Kind<1>{}, a.z, a.n_out, NO, z, Kind<DZ_ITEMS>{});
+			else items(row0, Kind<2>{}, a.z, a.n_out, NO, z, Kind<DZ_ITEMS>{});
+		}
+		if (a.dw_part) {
+			if (a.x.v) items(row0, Kind<1>{}, a.x, a.n_in, NI, x, Kind<X_ITEMS>{});
+			else items(row0, Kind<2>{}, a.x, a.n_in, NI, x, Kind<X_ITEMS>{});
+		}
+	};
+	const size_t chunks = (a.n + ROWS - 1) / ROWS;
+	if (blockIdx.x < chunks) ask((size_t)blockIdx.x * ROWS);
+	for (size_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+		const size_t row0 = chunk * ROWS;
+		__syncthreads();  // the last rows have been read
+#pragma unroll
+		for (int k = 0; k < DZ_ITEMS; ++k) {
+			const uint32_t item = tid + k * 256u, r = item / (NO / 8u), c = item % (NO / 8u);
+			float v[8], s[8];
+			a.dy.widen8_values(dy[k], v);
+			if (a.act != NGP_ACT_NONE) {
+				a.z.widen8(z[k], s);
+				act_slopes(a.act, s);
+#pragma unroll
+				for (int e = 0; e < 8; ++e) v[e] *= s[e];
+			}
+			v8<T> h;
+#pragma unroll
+			for (int e = 0; e < 8; ++e) {
+				v[e] = row0 + r < a.n && c * 8u + e < a.n_out ? v[e] : 0.0f;
+				db[e] += v[e];
+				h[e] = narrow<T>(v[e]);
+			}
+			*reinterpret_cast<s16x8*>(lds_dz + place(r, c, NO)) = __builtin_bit_cast(s16x8, h);
+		}
+		if (a.dw_part)
+#pragma unroll
+			for (int k = 0; k < X_ITEMS; ++k) {
+				const uint32_t item = tid + k * 256u, r = item / (NI / 8u), c = item % (NI / 8u);
+				float v[8];
+				a.x.widen8(x[k], v);
+				act_values(a.x_act, v);
+				v8<T> h;
+#pragma unroll
+				for (int e = 0; e < 8; ++e) h[e] = row0 + r < a.n && c * 8u + e < a.n_in ? narrow<T>(v[e]) : narrow<T>(0.0f);
+				*reinterpret_cast<s16x8*>(lds_x + place(r, c, NI)) = __builtin_bit_cast(s16x8, h);
+			}
+		__syncthreads();
+		if (chunk + gridDim.x < chunks) ask(row0 + (size_t)gridDim.x * ROWS);
+
+		if (a.dx) {
+			f32x16 c[NT] = {};
+#pragma unroll
+			for (int s = 0; s < NO / 16; ++s) {
+				const s16x8 p = *reinterpret_cast<const s16x8*>(lds_dz + place(strip * 32u + (lane & 31u), s * 2u + (lane >> 5), NO));
+#pragma unroll
+				for (int t = 0; t < NT; ++t) c[t] = mfma(T{}, w[t][s], p, c[t]);
+			}
+			const size_t i = row0 + strip * 32u + (lane & 31u);
+#pragma unroll
+			for (int t = 0; t < NT; ++t)
+#pragma unroll
+				for (int h = 0; h < 2; ++h) {
+					const uint32_t j = (nt0 + t) * 32u + 16u * h + 8u * (lane >> 5);
+					float v[8];
+					eight(c[t], h, v);
+					if (i >= a.n || j >= a.n_in) continue;
+					if (a.x_act != NGP_ACT_NONE) {
+						float s[8];
+						a.x.at8(i, j, a.n_in - j, s);
+						act_slopes(a.x_act, s);
+#pragma unroll
+						for (int k = 0; k < 8; ++k) v[k] *= s[k];
+					}
+					store8(a.dx + i * a.dx_stride + j, a.n_in - j, v);
+				}
+		}
+		if (a.dw_part)
+#pragma unroll
+			for (int s = 0; s < ROWS / 16; ++s) {
+				const s16x8 p = transposed(lds_dz, NO, s, wave % MW);
+#pragma unroll
+				for (int t = 0; t < WT; ++t) dw[t] = mfma(T{}, transposed(lds_x, NI, s, (wave + 4u * t) / MW), p, dw[t]);
+			}
+	}
+
+	if (a.dw_part)
+#pragma unroll
+		for (int t = 0; t < WT; ++t)
+#pragma unroll
+			for (int h = 0; h < 2; ++h) {
+				const uint32_t i = wave % MW * 32u + (lane & 31u), j = (wave + 4u * t) / MW * 32u + 16u * h + 8u * (lane >> 5);
+				const uint32_t n8 = (a.n_in + 7u) & ~7u;
+				float v[8];
+				eight(dw[t], h, v);
+				if (i < a.n_out && j < n8) store8(a.dw_part + ((size_t)blockIdx.x * a.n_out + i) * n8 + j, 8, v);
+			}
+	if (!a.db_part) return;
+	// the threads that share columns: every NO / 8-th
+	float* sums = reinterpret_cast<float*>(lds);
+	__syncthreads();
+#pragma unroll
+	for (int e = 0; e < 8; ++e) sums[tid * 9 + e] = db[e];
+	__syncthreads();
+	if (tid >= NO || tid >= a.n_out) return;
+	float total = 0.0f;
+	for (uint32_t o = tid / 8u; o < 256u; o += NO / 8u) total += sums[o * 9 + tid % 8u];
+	a.db_part[(size_t)blockIdx.x * a.n_out + tid] = total;
 }
 
 // ---- operands that do not lie as the product wants them ---------------------------------------------------------------
@@ -685,6 +896,16 @@ static void launch_product(void (*kernel)(ProductArgs, Out), uint32_t threads, u
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
+// The more splits there are, and the fewer sums, the more threads share one's splits: about four each.
+template <class T, class Out>
+static void join(const float* partial, uint32_t splits, size_t M, uint32_t N, const Out& out, hipStream_t s) {
+	const size_t items = M * ((N + 31u) / 32u * 4u);
+	uint32_t lines = 1;
+	while (lines < 32 && lines * 4 < splits && items * lines < 262144) lines *= 2;
+	k_product_join<T, Out><<<(uint32_t)((items * lines + 255) / 256), 256, 0, s>>>(partial, splits, M, N, lines, out);
+	NGP_HIP_CHECK(hipGetLastError());
+}
+
 // C[M][N] = P Q^T to `out`; a Room that does not run only counts what it takes.
 template <class T, class Out, bool P_BY_K, bool Q_BY_K>
 static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size_t K, const Out& out, Room& room, hipStream_t s) {
@@ -697,9 +918,7 @@ static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size
 	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128>, PRODUCT_THREADS, 65536, a, out, s);
 	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64>, PRODUCT_THREADS, 32768, a, out, s);
 	if (plan.splits > 1) {
-		const size_t items = M * ((N + 31u) / 32u * 4u);
-		k_product_join<T, Out><<<(uint32_t)((items + 255) / 256), 256, 0, s>>>(a.partial, plan.splits, M, N, out);
-		NGP_HIP_CHECK(hipGetLastError());
+		join<T>(a.partial, plan.splits, M, N, out, s);
 	}
 }
 
@@ -734,8 +953,39 @@ static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) 
 	return room.bytes;
 }
 
+// Narrow layers in one pass, where there are rows enough for every CU's first turn.  Two workgroups per CU of the smallest
+// kind; the larger ones keep more of dW in registers and leave more of it behind, one per CU does.
+constexpr uint32_t NARROW_WIDTH = 128, NARROW_ROWS = 16384;
+template <class T, int NI, int NO>
+static void launch_narrow(const NarrowArgs<T>& a, uint32_t grid, hipStream_t s) {
+	auto kernel = a.n_in % 8 == 0 && a.n_out % 8 == 0 ? k_narrow_backward<T, NI, NO, true> : k_narrow_backward<T, NI, NO, false>;
+	kernel<<<grid, 256, 0, s>>>(a);
+	NGP_HIP_CHECK(hipGetLastError());
+}
+template <class T>
+static size_t narrow_backward(const ngp_linear_backward_args& a, bool run, hipStream_t s) {
+	Room room{static_cast<char*>(a.workspace), run};
+	const bool ni = a.n_in > 64, no = a.n_out > 64;
+	const uint32_t grid = ni && no ? 256 : 512;
+	NarrowArgs<T> p{kept<T>(a.dy, a.dy_stride, {}), kept<T>(a.z, a.z_stride, a.z8), kept<T>(a.x, a.x_stride, a.x8), a.activation,
+	                a.x_activation, static_cast<const T*>(a.weights), a.weights_stride, a.n, a.n_in, a.n_out, static_cast<T*>(a.dx),
+	                a.dx_stride, nullptr, nullptr};
+	if (a.dweights) p.dw_part = room.take<float>((size_t)grid * a.n_out * up8(a.n_in));
+	if (a.dbias) p.db_part = room.take<float>((size_t)grid * a.n_out);
+	if (!run) return room.bytes;
+	if (ni && no) launch_narrow<T, 128, 128>(p, grid, s);
+	else if (ni) launch_narrow<T, 128, 64>(p, grid, s);
+	else if (no) launch_narrow<T, 64, 128>(p, grid, s);
+	else launch_narrow<T, 64, 64>(p, grid, s);
+	if (a.dweights)
+		join<T>(p.dw_part, grid, a.n_out, a.n_in, WeightsOut<T>{a.dweights, a.dweights_stride, a.dweights_type == NGP_TYPE_F32, a.accumulate != 0}, s);
+	if (a.dbias) launch_column_sums(p.db_part, grid, a.n_out, a.n_out, a.dbias, nullptr, a.accumulate != 0, s);
+	return room.bytes;
+}
+
 template <class T>
 static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipStream_t s) {
+	if (a.n >= NARROW_ROWS && a.n_in <= NARROW_WIDTH && a.n_out <= NARROW_WIDTH && (a.dx || a.dweights)) return narrow_backward<T>(a, run, s);
 	Room room{static_cast<char*>(a.workspace), run};
 	const bool products = a.dx || a.dweights, active = a.activation != NGP_ACT_NONE;
 	const Kept<T> dy = kept<T>(a.dy, a.dy_stride, {}), x = kept<T>(a.x, a.x_stride, a.x8);

@@ -196,6 +196,37 @@ def test_backward(n, n_in, n_out, kind):
         check_backward(kind, got, dy, x, z, w, name, x_name)
 
 
+# layers of up to 128 x 128 over many rows: every pair of padded widths, rows that end inside a workgroup's turn
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n, n_in, n_out", [(16384, 64, 64), (16385, 16, 16), (20011, 128, 128), (40001, 33, 67), (17000, 100, 64), (16500, 3, 120),
+                                            (16999, 128, 8), (100003, 1, 1)])
+def test_backward_of_narrow_layers(n, n_in, n_out, kind):
+    for seed, (name, x_name, z8, x8) in enumerate((("relu", "none", False, False), ("silu", "gelu", True, True), ("none", "relu", False, True))):
+        dy, xk, zk, w, x, z = backward_inputs(kind, n, n_in, n_out, seed, z8, x8)
+        every = U.call_linear_backward(kind, dy, xk, w, name, zk if name != "none" else None, x_name)
+        check_backward(kind, every, dy, x, z, w, name, x_name)
+    for k in range(3):
+        some = U.call_linear_backward(kind, dy, xk, w, name, None, x_name, dx=k == 0 or None, dw=k == 1 or None, db=k == 2 or None)
+        if k < 2:
+            assert torch.equal(some[k], every[k])
+        else:
+            check_backward(kind, some, dy, x, z, w, name, x_name)
+    base = normal(9, n_out, n_in), normal(10, n_out)
+    got = U.call_linear_backward(kind, dy, xk, w, name, None, x_name, dw_kind="f32", accumulate=True, dw=base[0].clone(), db=base[1].clone())
+    check_backward(kind, got, dy, x, z, w, name, x_name, "f32", base)
+
+
+def test_backward_of_narrow_layers_strides_and_frames():
+    t, nan = torch.float16, float("nan")
+    for n, n_in, n_out, pad, offset in ((16400, 64, 40, 8, 0), (16400, 72, 64, 3, 1), (17001, 45, 91, 0, 1)):
+        dy, x, z, w, dx, dw = (U.Framed(*s, t, pad, offset, value=nan, init=normal(k, *s, scale=0.2)) for k, s in enumerate(
+            ((n, n_out), (n, n_in), (n, n_out), (n_out, n_in), (n, n_in), (n_out, n_in))))
+        got = U.call_linear_backward("f16", dy.t, x.t, w.t, "gelu", z.t, "silu", dx=dx.t, dw=dw.t)
+        check_backward("f16", got, dy.t, x.t.double(), z.t.double(), w.t, "gelu", "silu")
+        for m in (dy, x, z, w, dx, dw):
+            assert m.untouched_outside()
+
+
 @pytest.mark.parametrize("n, n_in, n_out", [(1, 72, 40), (37, 40, 88), (70, 33, 67), (700, 200, 264)])
 def test_backward_accumulates_in_32_bits(n, n_in, n_out):
     dy, xk, zk, w, x, z = backward_inputs("f16", n, n_in, n_out, 5, True, False)
