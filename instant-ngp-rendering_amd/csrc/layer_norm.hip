@@ -246,36 +246,6 @@ __global__ void __launch_bounds__(256) k_norm_backward_columns(ngp_layer_norm_ba
 	}
 }
 
-// 16 columns by 64 shares at a time, four reads on their way; a wave's four shares meet by lane exchange, the 16 waves in LDS.
-__global__ void __launch_bounds__(1024) k_column_sums(const float* __restrict__ part, uint32_t shares, uint32_t columns, uint32_t width,
-                                                      float* out0, float* out1, bool accumulate) {
-	const uint32_t c = threadIdx.x % 16u, line = threadIdx.x / 16u, j = blockIdx.x * 16u + c;
-	float sum[4] = {};
-	if (j < columns)
-		for (uint32_t k = line; k < shares; k += 256u)
-#pragma unroll
-			for (uint32_t u = 0; u < 4; ++u)
-				if (k + 64u * u < shares) sum[u] += part[(size_t)(k + 64u * u) * columns + j];
-	float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-	v += __shfl_xor(v, 16);
-	v += __shfl_xor(v, 32);
-	__shared__ float s[16][16];
-	if (threadIdx.x % 64u < 16u) s[threadIdx.x / 64u][c] = v;
-	__syncthreads();
-	if (line || j >= columns) return;
-	v = 0.0f;
-	for (int w = 0; w < 16; ++w) v += s[w][c];
-	float* out = j < width ? out0 : out1;
-	const uint32_t o = j < width ? j : j - width;
-	if (out) out[o] = accumulate ? out[o] + v : v;
-}
-
-void launch_column_sums(const float* part, uint32_t shares, uint32_t columns, uint32_t width, float* out0, float* out1, bool accumulate,
-                        hipStream_t s) {
-	k_column_sums<<<(columns + 15) / 16, 1024, 0, s>>>(part, shares, columns, width, out0, out1, accumulate);
-	NGP_HIP_CHECK(hipGetLastError());
-}
-
 // A row's group: with many rows the smallest that holds the row in `most` chunks per thread (a wave's exchanges cost less
 // than barriers); with fewer rows than fill the GPU's 1024 SIMDs twice the largest that leaves every thread a chunk.
 struct NormShape {
@@ -347,7 +317,7 @@ static void norm_backward(const ngp_layer_norm_backward_args& a, hipStream_t s) 
 		k_norm_backward_rows<T><<<a.n, 1024, 0, s>>>(a);
 		NGP_HIP_CHECK(hipGetLastError());
 	}
-	if (part) launch_column_sums(part, p.parts, 2 * a.width, a.width, a.dgamma, a.dbeta, a.accumulate != 0, s);
+	if (part) launch_column_sums(part, p.parts, 2 * a.width, PutSums{a.dgamma, a.dbeta, a.width, a.accumulate != 0}, s);
 }
 
 void run_layer_norm_forward(const ngp_layer_norm_args& a, hipStream_t s) {

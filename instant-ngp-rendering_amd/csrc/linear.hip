@@ -583,6 +583,7 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 	const bool in = i < M && j < N;
 	float v[8] = {};
 	if (in)
+#pragma unroll 4
 		for (uint32_t s = line; s < splits; s += lines) {
 			float x[8];
 			load8(partial + ((size_t)s * M + i) * n8 + j, 8, x);
@@ -620,12 +621,13 @@ struct NarrowArgs {
 	uint32_t n_in, n_out;
 	T* dx;
 	size_t dx_stride;
-	float *dw_part, *db_part;  // [workgroup][n_out][n_in up to 8], [workgroup][n_out]
+	float* part;               // [workgroup][n_out][n_in up to 8], then n_out sums of dz
+	bool want_dw;
 };
 
 template <class T, int NI, int NO, bool EVEN>
-__global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(NarrowArgs<T> a) {
-	constexpr int ROWS = NI + NO > 128 ? 64 : 128;
+__global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : NI + NO > 128 ? 2 : 3) k_narrow_backward(NarrowArgs<T> a) {
+	constexpr int ROWS = 64;
 	constexpr int DZ_ITEMS = ROWS * NO / 8 / 256, X_ITEMS = ROWS * NI / 8 / 256;  // eights per thread
 	constexpr int STRIPS = ROWS / 32, NT = NI / 32 / (4 / STRIPS);               // a wave's strip of dx: NT tiles of 32 columns
 	constexpr int MW = NO / 32, WT = MW * (NI / 32) / 4;                           // dW: rows of tiles, tiles per wave
@@ -659,9 +661,10 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 #pragma unroll
 			for (int s = 0; s < NO / 16; ++s)
 #pragma unroll
-				for (int k = 0; k < 8; ++k) {
+				for (int k = 0; k < 8; ++k) {  // (no branch among the loads: what is not there is read as another and dropped)
 					const uint32_t row = (nt0 + t) * 32u + (lane & 31u), out = s * 16u + 8u * (lane >> 5) + k;
-					if (row < a.n_in && out < a.n_out) w[t][s][k] = __builtin_bit_cast(short, a.w[out * a.w_stride + row]);
+					const T v = a.w[min(out, a.n_out - 1u) * a.w_stride + min(row, a.n_in - 1u)];
+					w[t][s][k] = row < a.n_in && out < a.n_out ? __builtin_bit_cast(short, v) : (short)0;
 				}
 
 	f32x16 dw[WT] = {};
@@ -688,7 +691,7 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 			if (a.z.v) items(row0, Kind<1>{}, a.z, a.n_out, NO, z, Kind<DZ_ITEMS>{});
 			else items(row0, Kind<2>{}, a.z, a.n_out, NO, z, Kind<DZ_ITEMS>{});
 		}
-		if (a.dw_part) {
+		if (a.want_dw) {
 			if (a.x.v) items(row0, Kind<1>{}, a.x, a.n_in, NI, x, Kind<X_ITEMS>{});
 			else items(row0, Kind<2>{}, a.x, a.n_in, NI, x, Kind<X_ITEMS>{});
 		}
@@ -710,15 +713,16 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 				for (int e = 0; e < 8; ++e) v[e] *= s[e];
 			}
 			v8<T> h;
+			const bool in = row0 + r < a.n && c * 8u < a.n_out;
 #pragma unroll
 			for (int e = 0; e < 8; ++e) {
-				v[e] = row0 + r < a.n && c * 8u + e < a.n_out ? v[e] : 0.0f;
+				v[e] = in && (EVEN || c * 8u + e < a.n_out) ? v[e] : 0.0f;
 				db[e] += v[e];
 				h[e] = narrow<T>(v[e]);
 			}
 			*reinterpret_cast<s16x8*>(lds_dz + place(r, c, NO)) = __builtin_bit_cast(s16x8, h);
 		}
-		if (a.dw_part)
+		if (a.want_dw)
 #pragma unroll
 			for (int k = 0; k < X_ITEMS; ++k) {
 				const uint32_t item = tid + k * 256u, r = item / (NI / 8u), c = item % (NI / 8u);
@@ -726,8 +730,9 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 				a.x.widen8(x[k], v);
 				act_values(a.x_act, v);
 				v8<T> h;
+				const bool in = row0 + r < a.n && c * 8u < a.n_in;
 #pragma unroll
-				for (int e = 0; e < 8; ++e) h[e] = row0 + r < a.n && c * 8u + e < a.n_in ? narrow<T>(v[e]) : narrow<T>(0.0f);
+				for (int e = 0; e < 8; ++e) h[e] = narrow<T>(in && (EVEN || c * 8u + e < a.n_in) ? v[e] : 0.0f);
 				*reinterpret_cast<s16x8*>(lds_x + place(r, c, NI)) = __builtin_bit_cast(s16x8, h);
 			}
 		__syncthreads();
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 					store8(a.dx + i * a.dx_stride + j, a.n_in - j, v);
 				}
 		}
-		if (a.dw_part)
+		if (a.want_dw)
 #pragma unroll
 			for (int s = 0; s < ROWS / 16; ++s) {
 				const s16x8 p = transposed(lds_dz, NO, s, wave % MW);
@@ -769,18 +774,18 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 			}
 	}
 
-	if (a.dw_part)
+	const uint32_t n8 = (a.n_in + 7u) & ~7u;
+	float* part = a.part + (size_t)blockIdx.x * a.n_out * (n8 + 1u);
+	if (a.want_dw)
 #pragma unroll
 		for (int t = 0; t < WT; ++t)
 #pragma unroll
 			for (int h = 0; h < 2; ++h) {
 				const uint32_t i = wave % MW * 32u + (lane & 31u), j = (wave + 4u * t) / MW * 32u + 16u * h + 8u * (lane >> 5);
-				const uint32_t n8 = (a.n_in + 7u) & ~7u;
 				float v[8];
 				eight(dw[t], h, v);
-				if (i < a.n_out && j < n8) store8(a.dw_part + ((size_t)blockIdx.x * a.n_out + i) * n8 + j, 8, v);
+				if (i < a.n_out && j < n8) store8(part + i * n8 + j, 8, v);
 			}
-	if (!a.db_part) return;
 	// the threads that share columns: every NO / 8-th
 	float* sums = reinterpret_cast<float*>(lds);
 	__syncthreads();
@@ -790,8 +795,29 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(
 	if (tid >= NO || tid >= a.n_out) return;
 	float total = 0.0f;
 	for (uint32_t o = tid / 8u; o < 256u; o += NO / 8u) total += sums[o * 9 + tid % 8u];
-	a.db_part[(size_t)blockIdx.x * a.n_out + tid] = total;
+	part[a.n_out * n8 + tid] = total;
 }
+
+// A column of those shares to where it belongs.
+template <class T>
+struct PutNarrow {
+	void* dw;
+	size_t stride;
+	bool f32, accumulate;
+	uint32_t n_in, n_out;
+	float* db;
+	__device__ __forceinline__ void operator()(size_t c, float v) const {
+		const uint32_t n8 = (n_in + 7u) & ~7u, i = (uint32_t)c / n8, j = (uint32_t)c % n8;
+		if (i >= n_out) {
+			float* d = db + (c - n_out * n8);
+			if (db) *d = accumulate ? *d + v : v;
+		} else if (dw && j < n_in) {
+			float* d = static_cast<float*>(dw) + i * stride + j;
+			if (f32) *d = accumulate ? *d + v : v;
+			else static_cast<T*>(dw)[i * stride + j] = narrow<T>(v);
+		}
+	}
+};
 
 // ---- operands that do not lie as the product wants them ---------------------------------------------------------------
 // act(v), rounded to T, in rows of `width` up to 8, filled up with zeros.
@@ -953,8 +979,8 @@ static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) 
 	return room.bytes;
 }
 
-// Narrow layers in one pass, where there are rows enough for every CU's first turn.  Two workgroups per CU of the smallest
-// kind; the larger ones keep more of dW in registers and leave more of it behind, one per CU does.
+// Narrow layers in one pass, where there are rows enough for every CU's first turn: two workgroups per CU, for 128 x 128 (with
+// four times the sums to leave behind) one.
 constexpr uint32_t NARROW_WIDTH = 128, NARROW_ROWS = 16384;
 template <class T, int NI, int NO>
 static void launch_narrow(const NarrowArgs<T>& a, uint32_t grid, hipStream_t s) {
@@ -967,19 +993,19 @@ static size_t narrow_backward(const ngp_linear_backward_args& a, bool run, hipSt
 	Room room{static_cast<char*>(a.workspace), run};
 	const bool ni = a.n_in > 64, no = a.n_out > 64;
 	const uint32_t grid = ni && no ? 256 : 512;
-	NarrowArgs<T> p{kept<T>(a.dy, a.dy_stride, {}), kept<T>(a.z, a.z_stride, a.z8), kept<T>(a.x, a.x_stride, a.x8), a.activation,
-	                a.x_activation, static_cast<const T*>(a.weights), a.weights_stride, a.n, a.n_in, a.n_out, static_cast<T*>(a.dx),
-	                a.dx_stride, nullptr, nullptr};
-	if (a.dweights) p.dw_part = room.take<float>((size_t)grid * a.n_out * up8(a.n_in));
-	if (a.dbias) p.db_part = room.take<float>((size_t)grid * a.n_out);
+	const size_t columns = (size_t)a.n_out * (up8(a.n_in) + 1);
+	float* part = room.take<float>(grid * columns);
 	if (!run) return room.bytes;
+	const NarrowArgs<T> p{kept<T>(a.dy, a.dy_stride, {}), kept<T>(a.z, a.z_stride, a.z8), kept<T>(a.x, a.x_stride, a.x8), a.activation,
+	                      a.x_activation, static_cast<const T*>(a.weights), a.weights_stride, a.n, a.n_in, a.n_out,
+	                      static_cast<T*>(a.dx), a.dx_stride, part, a.dweights != nullptr};
 	if (ni && no) launch_narrow<T, 128, 128>(p, grid, s);
 	else if (ni) launch_narrow<T, 128, 64>(p, grid, s);
 	else if (no) launch_narrow<T, 64, 128>(p, grid, s);
 	else launch_narrow<T, 64, 64>(p, grid, s);
-	if (a.dweights)
-		join<T>(p.dw_part, grid, a.n_out, a.n_in, WeightsOut<T>{a.dweights, a.dweights_stride, a.dweights_type == NGP_TYPE_F32, a.accumulate != 0}, s);
-	if (a.dbias) launch_column_sums(p.db_part, grid, a.n_out, a.n_out, a.dbias, nullptr, a.accumulate != 0, s);
+	if (a.dweights || a.dbias)
+		launch_column_sums(part, grid, columns, PutNarrow<T>{a.dweights, a.dweights_stride, a.dweights_type == NGP_TYPE_F32,
+		                                                     a.accumulate != 0, a.n_in, a.n_out, a.dbias}, s);
 	return room.bytes;
 }
 
@@ -1005,7 +1031,7 @@ static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipSt
 			k_linear_dz<T><<<dim3(wide, shares), 256, 0, s>>>(dy, kept<T>(a.z, a.z_stride, a.z8), a.activation, a.n, a.n_out, groups, each,
 			                                                 dz_to, part);
 			NGP_HIP_CHECK(hipGetLastError());
-			if (a.dbias) launch_column_sums(part, shares, a.n_out, a.n_out, a.dbias, nullptr, a.accumulate != 0, s);
+			if (a.dbias) launch_column_sums(part, shares, a.n_out, PutSums{a.dbias, nullptr, a.n_out, a.accumulate != 0}, s);
 		}
 	}
 	if (a.dx && a.n) {
