@@ -271,19 +271,6 @@ struct Fragments {
 	}
 };
 
-// Asks the compiler's scheduler for an even mixture of the LDS reads, the loads and the matrix instructions that stand
-// before it, instead of one kind after the other.
-template <int READS, int LOADS, int PRODUCTS>
-__device__ __forceinline__ void alternate() {
-	if constexpr (PRODUCTS > 0) {
-		constexpr int reads = (READS + PRODUCTS - 1) / PRODUCTS, loads = (LOADS + PRODUCTS - 1) / PRODUCTS;
-		if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
-		if constexpr (loads > 0) __builtin_amdgcn_sched_group_barrier(0x010, loads, 0);
-		__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-		alternate<READS - reads, LOADS - loads, PRODUCTS - 1>();
-	}
-}
-
 // Eight neighbouring columns of C (j a multiple of 8, `left` of them and more up to the row's end; 0: none) to the caller's
 // matrices.  The four lanes of a block of 32 call it together.
 template <class T, class Out>
@@ -402,16 +389,27 @@ struct WriteOut {
 	}
 };
 
-// BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through two LDS buffers: while the matrix cores
-// work on one stage, the next is on its way from memory into the other buffer without passing registers.  P's rows are
-// the matrix instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
-template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN>
+// s_waitcnt's operand: vmcnt and lgkmcnt (15: any), expcnt any.
+constexpr int waits(int vmcnt, int lgkmcnt) { return (vmcnt & 15) | 7 << 4 | lgkmcnt << 8 | (vmcnt >> 4) << 14; }
+// Nothing moves over this point, in the compiler or among the waves.
+__device__ __forceinline__ void meet() {
+	asm volatile("" ::: "memory");
+	__builtin_amdgcn_sched_barrier(0);
+	__builtin_amdgcn_s_barrier();
+	__builtin_amdgcn_sched_barrier(0);
+	asm volatile("" ::: "memory");
+}
+
+// BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through BUFFERS LDS buffers: while the matrix cores
+// work on one stage, the others are on their way from memory into LDS without passing registers.  P's rows are the matrix
+// instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN, int BUFFERS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, Out out) {
 	constexpr int TM = BM / 64, TN = BN / 64;  // 32 x 32 tiles per wave
 	typedef Stage<T, BM, P_BY_K, 64, PRODUCT_THREADS> PStage;
 	typedef Stage<T, BN, Q_BY_K, 64, PRODUCT_THREADS> QStage;
-	constexpr int STAGE = PStage::BYTES + QStage::BYTES;
-	static_assert(4 * STRIP<TN> * 4 <= 2 * STAGE, "the stages' LDS holds the strips");
+	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
+	static_assert(4 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
 	extern __shared__ __attribute__((aligned(16))) char lds[];
 
 	const Place<BM, BN> at(a);
@@ -430,51 +428,41 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, O
 		qs.begin(a.q, at.n0, a.N, at.k0, a.K);
 		pf.begin(wm);
 		qf.begin(wn);
-		constexpr int READS = TM * (P_BY_K ? 2 : 1) + TN * (Q_BY_K ? 2 : 1), LOADS = PStage::LOADS + QStage::LOADS;
-		s16x8 p[2][TM], q[2][TN];
-		auto read = [&](const char* from, int k) {
-#pragma unroll
-			for (int t = 0; t < TN; ++t) q[k & 1][t] = qf.read(from + PStage::BYTES, k, t);
-#pragma unroll
-			for (int t = 0; t < TM; ++t) p[k & 1][t] = pf.read(from, k, t);
-		};
-		auto multiply = [&](int k) {
-#pragma unroll
-			for (int n = 0; n < TN; ++n)
-#pragma unroll
-				for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k & 1][n], p[k & 1][m], c[n][m]);
-		};
-		auto arrived = [] {  // this wave's reads of the one buffer are done and its loads into the other there; then everybody's
-			__builtin_amdgcn_s_waitcnt(0);
-			__syncthreads();
+		uint32_t to = 0, now = 0;
+		auto next = [](uint32_t at) { return at == (BUFFERS - 1) * STAGE ? 0u : at + STAGE; };
+		auto load = [&](bool more) {
+			ps.load(lds + to, more);
+			qs.load(lds + to + PStage::BYTES, more);
+			to = next(to);
 		};
 		// the part of K that fills no stage comes first, so that the loop has whole stages only
 		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % 64u) + 1u;
 		ps.load_first(lds, k_in);
 		qs.load_first(lds + PStage::BYTES, k_in);
-		arrived();
-		ps.load(lds + STAGE, stages > 1);
-		qs.load(lds + STAGE + PStage::BYTES, stages > 1);
-		read(lds, 0);
-		uint32_t now = 0;
-		for (uint32_t s = 1; s < stages; ++s, now ^= STAGE) {
+		to = next(to);
 #pragma unroll
-			for (int k = 0; k < 3; ++k) {
-				read(lds + now, k + 1);
-				multiply(k);
-				alternate<READS, 0, TM * TN>();
+		for (uint32_t s = 1; s < BUFFERS - 1; ++s) load(s < stages);
+		for (uint32_t s = 0; s < stages; ++s, now = next(now)) {
+			// stage s has arrived, as far as this wave asked for it, and its reads of stage s - 1 are done; then everybody's
+			__builtin_amdgcn_s_waitcnt(waits((BUFFERS - 2) * LOADS, 0));
+			meet();
+			load(s + BUFFERS - 1 < stages);
+			s16x8 p[2][TM], q[2][TN];
+			auto read = [&](int k) {
+#pragma unroll
+				for (int t = 0; t < TN; ++t) q[k & 1][t] = qf.read(lds + now + PStage::BYTES, k, t);
+#pragma unroll
+				for (int t = 0; t < TM; ++t) p[k & 1][t] = pf.read(lds + now, k, t);
+			};
+			read(0);
+#pragma unroll
+			for (int k = 0; k < 4; ++k) {
+				if (k < 3) read(k + 1);
+#pragma unroll
+				for (int n = 0; n < TN; ++n)
+#pragma unroll
+					for (int m = 0; m < TM; ++m) c[n][m] = mfma(T{}, q[k & 1][n], p[k & 1][m], c[n][m]);
 			}
-			arrived();
-			ps.load(lds + now, s + 1 < stages);
-			qs.load(lds + now + PStage::BYTES, s + 1 < stages);
-			read(lds + (now ^ STAGE), 0);
-			multiply(3);
-			alternate<READS, LOADS, TM * TN>();
-		}
-#pragma unroll
-		for (int k = 0; k < 4; ++k) {
-			if (k < 3) read(lds + now, k + 1);
-			multiply(k);
 		}
 		__builtin_amdgcn_s_waitcnt(0);
 	}
@@ -516,18 +504,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 			ps.load(to, s < stages);
 			qs.load(to + PStage::BYTES, s < stages);
 		};
-		// nothing moves over this point, in the compiler or among the waves
-		auto meet = [] {
-			asm volatile("" ::: "memory");
-			__builtin_amdgcn_sched_barrier(0);
-			__builtin_amdgcn_s_barrier();
-			__builtin_amdgcn_sched_barrier(0);
-			asm volatile("" ::: "memory");
-		};
-		// s_waitcnt with lgkmcnt = 0, this wave's reads are done, and with vmcnt either 63, any loads may be on their way, or
-		// such that all but the latest BUFFERS - 2 stages it asked for are there
-		constexpr int READ = 15 | 7 << 4 | 3 << 14, ARRIVED = (BUFFERS - 2) * LOADS | 7 << 4;
-		static_assert((BUFFERS - 2) * LOADS < 16, "vmcnt's low field");
+		// all but the latest BUFFERS - 2 stages a wave asked for are there, and its reads are done
+		constexpr int ARRIVED = waits((BUFFERS - 2) * LOADS, 0), READ = waits(63, 0);
 		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % DEEP) + 1u;
 		ps.load_first(lds, k_in);
 		qs.load_first(lds + PStage::BYTES, k_in);
@@ -896,21 +874,37 @@ struct ProductPlan {
 	size_t k_each = 0;
 };
 
-// The tile: the largest that still gives most of the 256 CUs something to do (a 256 x 256 tile moves a quarter of the bytes
-// of a 64 x 64 one through LDS per multiplication).  K is split where the tiles are too few: until there are about two
-// workgroups per CU, or four stages each.
+// The tile and how often K is split: whichever pair should take least, in microseconds as measured over products of 32 to
+// 65536 rows (bf16, both operands along k; the estimate is within a quarter of the measured time).  With n workgroups per CU,
+// rounded up, a stage of 64 k takes max(least, n each): a 64 tile's loads and barriers take as long as two of it multiply
+// (1024^3: 8 us with 64 tiles, 12 with 128, 25 with 256), a 256 tile moves a quarter of the bytes per multiplication (4096 x
+// 2048 x 4096: 105, 70 and 60 us).  Splits write their sums and read them again at about 4.2 TB/s, in a launch of their own
+// (32 x 4096 x 4096: 19 us with 64 tiles, 12 with four splits; 2048 x 1024 x 1024: 10 us, 24 with two).
 static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
-	ProductPlan p;
-	auto tiles = [&](size_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-	p.tile = M > 128 && N > 128 && tiles(256) >= 192 ? 256 : (M > 64 && N > 64 && tiles(128) * (K / 512 + 1) >= 256 ? 128 : 64);
-	p.tiles_m = (uint32_t)((M + p.tile - 1) / p.tile);
-	p.tiles_n = (uint32_t)((N + p.tile - 1) / p.tile);
-	const size_t stages = (K + PRODUCT_K - 1) / PRODUCT_K, count = (size_t)p.tiles_m * p.tiles_n;
-	const size_t splits = count >= 256 ? 1 : std::max<size_t>(1, std::min<size_t>(std::min<size_t>(512 / count, stages / 4), 256));
-	const size_t each = std::max<size_t>(1, (stages + splits - 1) / splits);
-	p.k_each = each * PRODUCT_K;
-	p.splits = stages ? (uint32_t)((stages + each - 1) / each) : 1u;
-	return p;
+	struct Kind {
+		int tile;
+		double least, each;
+	};
+	ProductPlan best;
+	double least = 1e30;
+	const size_t stages = std::max<size_t>(1, (K + PRODUCT_K - 1) / PRODUCT_K);
+	for (const Kind& kind : {Kind{64, 0.23, 0.185}, Kind{128, 0.5, 0.52}, Kind{256, 1.3, 1.68}}) {
+		const size_t tiles = ((M + kind.tile - 1) / kind.tile) * (((size_t)N + kind.tile - 1) / kind.tile);
+		for (size_t splits = 1; splits <= std::min<size_t>(64, stages); splits *= 2) {
+			const size_t each = (stages + splits - 1) / splits, used = (stages + each - 1) / each;
+			const double n = (double)((tiles * used + 255) / 256);
+			const double join = used > 1 ? 3.0 + 8e-6 * (double)used * (double)M * N / 4.2 : 0.0;
+			const double t = 4.0 + 0.4 * n + each * std::max(kind.least, kind.each * n) + join;
+			if (t >= least) continue;
+			least = t;
+			best.tile = kind.tile;
+			best.splits = (uint32_t)used;
+			best.k_each = each * PRODUCT_K;
+		}
+	}
+	best.tiles_m = (uint32_t)((M + best.tile - 1) / best.tile);
+	best.tiles_n = (uint32_t)((N + best.tile - 1) / best.tile);
+	return best;
 }
 
 template <class Out>
@@ -941,8 +935,8 @@ static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size
 	if (plan.splits > 1) a.partial = room.take<float>((size_t)plan.splits * M * up8(N));
 	if (!room.run) return;
 	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, WIDE_THREADS, 131072, a, out, s);
-	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128>, PRODUCT_THREADS, 65536, a, out, s);
-	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64>, PRODUCT_THREADS, 32768, a, out, s);
+	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128, 2>, PRODUCT_THREADS, 2 * 32768, a, out, s);
+	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64, 3>, PRODUCT_THREADS, 3 * 16384, a, out, s);
 	if (plan.splits > 1) {
 		join<T>(a.partial, plan.splits, M, N, out, s);
 	}
