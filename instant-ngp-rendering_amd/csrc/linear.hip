@@ -584,6 +584,86 @@ __global__ void __launch_bounds__(256) k_product_join(const float* __restrict__ 
 	finish_block<T>(out, i, j, left, out.columns(j, left), fetched, v);
 }
 
+// ---- a few rows ---------------------------------------------------------------------------------------------------------
+// Forward for up to 16 rows, as a served network evaluates a query or a few: bound by the read of the weights, and for small
+// ones by latency, so one launch and no workspace.  A workgroup of eight waves takes FEATURES outputs and all rows; the waves
+// take 64 of k in turn, of which a lane reads 16 neighbouring ones (32 bytes of a weight's row and of a row of x, in whatever
+// alignment) for two matrix instructions: their k is permuted the same way in both operands.  The waves' sums meet in LDS.
+constexpr uint32_t FEW_ROWS = 16, FEW_THREADS = 512;
+__device__ __forceinline__ f32x4 mfma16(f16, s16x8 a, s16x8 b, f32x4 c) {
+	return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8<f16>, a), __builtin_bit_cast(v8<f16>, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bf16, s16x8 a, s16x8 b, f32x4 c) {
+	return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8<bf16>, a), __builtin_bit_cast(v8<bf16>, b), c, 0, 0, 0);
+}
+
+template <class T, int FEATURES>
+__global__ void __launch_bounds__(FEW_THREADS) k_few_rows(const T* __restrict__ x, size_t x_stride, const T* __restrict__ w, size_t w_stride,
+                                                          uint32_t n, uint32_t n_in, uint32_t n_out, ForwardOut<T> out) {
+	constexpr int TILES = FEATURES / 16, WAVES = FEW_THREADS / 64, AHEAD = 4;  // steps of 64 k whose reads go out together
+	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, row = lane & 15u, j0 = blockIdx.x * FEATURES;
+	// rows that are not there: the last one's values, whose sums nobody takes
+	const T* xr = x + min(row, n - 1u) * x_stride;
+	const T* wr[TILES];
+#pragma unroll
+	for (int t = 0; t < TILES; ++t) wr[t] = w + min(j0 + t * 16u + row, n_out - 1u) * w_stride;
+	f32x4 c[TILES] = {};
+	const uint32_t whole = n_in / 64u;
+	auto step = [&](uint32_t first, auto count) {  // `count` steps of this wave from step `first` on
+		v8<T> xv[count][2], wv[count][TILES][2];
+#pragma unroll
+		for (int u = 0; u < count; ++u) {
+			const uint32_t k = (first + u * WAVES) * 64u + (lane >> 4) * 16u;
+#pragma unroll
+			for (int h = 0; h < 2; ++h) {
+#pragma unroll
+				for (int t = 0; t < TILES; ++t) wv[u][t][h] = *reinterpret_cast<const v8<T>*>(wr[t] + k + 8 * h);
+				xv[u][h] = *reinterpret_cast<const v8<T>*>(xr + k + 8 * h);
+			}
+		}
+#pragma unroll
+		for (int u = 0; u < count; ++u)
+#pragma unroll
+			for (int h = 0; h < 2; ++h)
+#pragma unroll
+				for (int t = 0; t < TILES; ++t)
+					c[t] = mfma16(T{}, __builtin_bit_cast(s16x8, wv[u][t][h]), __builtin_bit_cast(s16x8, xv[u][h]), c[t]);
+	};
+	uint32_t s = wave;
+	for (; s + (AHEAD - 1) * WAVES < whole; s += AHEAD * WAVES) step(s, Kind<AHEAD>{});
+	for (; s < whole; s += WAVES) step(s, Kind<1>{});
+	if (n_in % 64u && whole % WAVES == wave) {  // the rest of k, filled up with zeros
+		const uint32_t k = whole * 64u + (lane >> 4) * 16u;
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			const uint32_t left = n_in > k + 8u * h ? n_in - k - 8u * h : 0u;
+			const v8<T> xv = load8_raw(xr + k + 8 * h, left);
+#pragma unroll
+			for (int t = 0; t < TILES; ++t)
+				c[t] = mfma16(T{}, __builtin_bit_cast(s16x8, load8_raw(wr[t] + k + 8 * h, left)), __builtin_bit_cast(s16x8, xv), c[t]);
+		}
+	}
+	// register r of a tile: output 4 (lane / 16) + r of row lane % 16
+	constexpr int PITCH = FEATURES + 4;
+	__shared__ __attribute__((aligned(16))) float sums[WAVES][16][PITCH];
+#pragma unroll
+	for (int t = 0; t < TILES; ++t) *reinterpret_cast<f32x4*>(&sums[wave][row][t * 16 + (lane >> 4) * 4]) = c[t];
+	__syncthreads();
+	if (threadIdx.x >= 16 * FEATURES / 8) return;
+	const uint32_t i = threadIdx.x / (FEATURES / 8), f = threadIdx.x % (FEATURES / 8) * 8u, j = j0 + f;
+	float v[8] = {};
+#pragma unroll
+	for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+		for (int e = 0; e < 8; ++e) v[e] += sums[k][i][f + e];
+	const uint32_t left = i < n && j < n_out ? n_out - j : 0u;
+#pragma unroll
+	for (int e = 0; e < 8; ++e) v[e] = (uint32_t)e < left ? v[e] : 0.0f;
+	typename ForwardOut<T>::Fetched fetched = {};
+	if (left) out.by_kind([&](auto kind) { fetched = out.fetch(kind, i, j, left); });
+	finish_block<T>(out, i, j, left, out.columns(j, left), fetched, v);
+}
+
 // ---- narrow layers ------------------------------------------------------------------------------------------------------
 // Backward of layers of up to 128 x 128 over many rows: memory bound, so all of it in one pass over dy, z and x.  Persistent
 // workgroups of four waves take ROWS rows at a time: dz and the layer's input go to LDS in 16 bits ([row][feature], from
@@ -965,10 +1045,21 @@ template <class T>
 static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) {
 	Room room{static_cast<char*>(a.workspace), run};
 	if (!a.n) return 0;
-	const Matrix x = operand<T>(kept<T>(a.x, a.x_stride, {}), NGP_ACT_NONE, a.n, a.n_in, room, s);
-	const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
 	const ForwardOut<T> out{a.bias, static_cast<const T*>(a.residual), static_cast<T*>(a.y), static_cast<T*>(a.z), a.z8,
 	                        a.residual_stride, a.y_stride, a.z_stride, a.activation};
+	if (a.n <= FEW_ROWS) {
+		// a block of 32 outputs per workgroup where a checkpoint's blocks are, or where that still gives most CUs one
+		if (!run) return 0;
+		const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.weights);
+		if (a.z8.q || a.n_out > 256 * 16)
+			k_few_rows<T, 32><<<(a.n_out + 31) / 32, FEW_THREADS, 0, s>>>(x, a.x_stride, w, a.weights_stride, a.n, a.n_in, a.n_out, out);
+		else
+			k_few_rows<T, 16><<<(a.n_out + 15) / 16, FEW_THREADS, 0, s>>>(x, a.x_stride, w, a.weights_stride, a.n, a.n_in, a.n_out, out);
+		NGP_HIP_CHECK(hipGetLastError());
+		return 0;
+	}
+	const Matrix x = operand<T>(kept<T>(a.x, a.x_stride, {}), NGP_ACT_NONE, a.n, a.n_in, room, s);
+	const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
 	product<T, ForwardOut<T>, false, false>(x, w, a.n, a.n_out, a.n_in, out, room, s);
 	return room.bytes;
 }
