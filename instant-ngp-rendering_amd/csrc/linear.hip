@@ -609,11 +609,11 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_rows(const T* __restrict__ 
 	for (int t = 0; t < TILES; ++t) wr[t] = w + min(j0 + t * 16u + row, n_out - 1u) * w_stride;
 	f32x4 c[TILES] = {};
 	const uint32_t whole = n_in / 64u;
-	auto step = [&](uint32_t first, auto count) {  // `count` steps of this wave from step `first` on
+	auto step = [&](uint32_t first, auto count) {  // `count` steps from step `first` on
 		v8<T> xv[count][2], wv[count][TILES][2];
 #pragma unroll
 		for (int u = 0; u < count; ++u) {
-			const uint32_t k = (first + u * WAVES) * 64u + (lane >> 4) * 16u;
+			const uint32_t k = (first + u) * 64u + (lane >> 4) * 16u;
 #pragma unroll
 			for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -629,9 +629,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_rows(const T* __restrict__ 
 				for (int t = 0; t < TILES; ++t)
 					c[t] = mfma16(T{}, __builtin_bit_cast(s16x8, wv[u][t][h]), __builtin_bit_cast(s16x8, xv[u][h]), c[t]);
 	};
-	uint32_t s = wave;
-	for (; s + (AHEAD - 1) * WAVES < whole; s += AHEAD * WAVES) step(s, Kind<AHEAD>{});
-	for (; s < whole; s += WAVES) step(s, Kind<1>{});
+	// AHEAD neighbouring steps at a time, 512 bytes of a row, then what is left of them one by one
+	uint32_t s = wave * AHEAD;
+	for (; s + AHEAD <= whole; s += AHEAD * WAVES) step(s, Kind<AHEAD>{});
+	for (uint32_t u = whole / AHEAD * AHEAD + wave; u < whole; u += WAVES) step(u, Kind<1>{});
 	if (n_in % 64u && whole % WAVES == wave) {  // the rest of k, filled up with zeros
 		const uint32_t k = whole * 64u + (lane >> 4) * 16u;
 #pragma unroll
@@ -952,6 +953,7 @@ struct ProductPlan {
 	int tile = 64;
 	uint32_t tiles_m = 0, tiles_n = 0, splits = 1;
 	size_t k_each = 0;
+	double us = 1e30;  // estimated
 };
 
 // The tile and how often K is split: whichever pair should take least, in microseconds as measured over products of 32 to
@@ -966,7 +968,6 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
 		double least, each;
 	};
 	ProductPlan best;
-	double least = 1e30;
 	const size_t stages = std::max<size_t>(1, (K + PRODUCT_K - 1) / PRODUCT_K);
 	for (const Kind& kind : {Kind{64, 0.23, 0.185}, Kind{128, 0.5, 0.52}, Kind{256, 1.3, 1.68}}) {
 		const size_t tiles = ((M + kind.tile - 1) / kind.tile) * (((size_t)N + kind.tile - 1) / kind.tile);
@@ -975,8 +976,8 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
 			const double n = (double)((tiles * used + 255) / 256);
 			const double join = used > 1 ? 3.0 + 8e-6 * (double)used * (double)M * N / 4.2 : 0.0;
 			const double t = 4.0 + 0.4 * n + each * std::max(kind.least, kind.each * n) + join;
-			if (t >= least) continue;
-			least = t;
+			if (t >= best.us) continue;
+			best.us = t;
 			best.tile = kind.tile;
 			best.splits = (uint32_t)used;
 			best.k_each = each * PRODUCT_K;
@@ -1047,14 +1048,18 @@ static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) 
 	if (!a.n) return 0;
 	const ForwardOut<T> out{a.bias, static_cast<const T*>(a.residual), static_cast<T*>(a.y), static_cast<T*>(a.z), a.z8,
 	                        a.residual_stride, a.y_stride, a.z_stride, a.activation};
-	if (a.n <= FEW_ROWS) {
-		// a block of 32 outputs per workgroup where a checkpoint's blocks are, or where that still gives most CUs one
+	// 16 outputs per workgroup; 32 where a checkpoint's blocks are, or where that still gives every CU one.  A CU reads the
+	// weights at 20 GB/s: with few outputs and a long K the product's splits use more of them (16 x 16384 x 1024: 30 us, 12).
+	const bool pairs = a.z8.q || a.n_out > 256 * 16;
+	const uint32_t groups = pairs ? (a.n_out + 31) / 32 : (a.n_out + 15) / 16;
+	const double few_us = 2.5 + 2.0 * a.n_in * a.n_out / (std::min(groups, 256u) * 20e3);
+	if (a.n <= FEW_ROWS && few_us <= plan_product(a.n, a.n_out, a.n_in).us) {
 		if (!run) return 0;
 		const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.weights);
-		if (a.z8.q || a.n_out > 256 * 16)
-			k_few_rows<T, 32><<<(a.n_out + 31) / 32, FEW_THREADS, 0, s>>>(x, a.x_stride, w, a.weights_stride, a.n, a.n_in, a.n_out, out);
+		if (pairs)
+			k_few_rows<T, 32><<<groups, FEW_THREADS, 0, s>>>(x, a.x_stride, w, a.weights_stride, a.n, a.n_in, a.n_out, out);
 		else
-			k_few_rows<T, 16><<<(a.n_out + 15) / 16, FEW_THREADS, 0, s>>>(x, a.x_stride, w, a.weights_stride, a.n, a.n_in, a.n_out, out);
+			k_few_rows<T, 16><<<groups, FEW_THREADS, 0, s>>>(x, a.x_stride, w, a.weights_stride, a.n, a.n_in, a.n_out, out);
 		NGP_HIP_CHECK(hipGetLastError());
 		return 0;
 	}
