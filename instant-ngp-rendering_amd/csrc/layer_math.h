@@ -24,12 +24,12 @@ __device__ __forceinline__ T narrow(float v) { return (T)v; }  // to nearest, ti
 __device__ __forceinline__ float act_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 __device__ __forceinline__ float act_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// The normal distribution by two polynomials of degree 8, fitted for the least largest error (one exponential each and no
-// division, half the cost of a rational form of the tail: a 256 x 256 tile's 65536 gelus are a quarter of its time at K = 2048):
-//  * the tail Phi(-a) = 2^L(a) for 0 <= a <= 8: relative error 5.3e-6, 1.1e-5 with fp32 rounding.  Past 8 nothing is left of
-//    it (6e-16).
-//  * the gelu's slope at -a, Phi(-a) - a phi(a) = exp(-a^2 / 2) S(a): off by 1.0e-6, and by less than 1e-8 past a = 6,
-//    where S(6) stands for S(a).
+// The normal distribution by a polynomial each, fitted for the least largest error (one exponential and no division, half the
+// cost of a rational form of the tail: a 256 x 256 tile's 65536 gelus are a quarter of its time at K = 2048):
+//  * the tail Phi(-a) = 2^L(a) for 0 <= a <= 8, degree 8: relative error 5.3e-6, 1.1e-5 with fp32 rounding.  Past 8 nothing
+//    is left of it (6e-16).
+//  * the gelu's slope at -a, Phi(-a) - a phi(a) = exp(-a^2 / 2) S(a), degree 9: off by 2.6e-7 (it enters sums over all rows,
+//    which are held in fp32), and by less than 6e-8 past a = 6, where S(6) stands for S(a).
 __device__ __forceinline__ float gelu_value(float z) {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
 	const float a = fminf(fabsf(z), 8.0f);
 	float l = 7.427881287228275e-08f;
@@ -45,15 +45,16 @@ __device__ __forceinline__ float gelu_value(float z) {  // z Phi(z) = max(z, 0) 
 }
 __device__ __forceinline__ float gelu_slope(float z) {
 	const float a = fminf(fabsf(z), 6.0f), bell = __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);  // -log2(e) / 2
-	float s = 3.790504420392107e-05f;
-	s = __builtin_fmaf(s, a, -0.0006154082213131475f);
-	s = __builtin_fmaf(s, a, 0.004399921135406666f);
-	s = __builtin_fmaf(s, a, -0.018825302738585882f);
-	s = __builtin_fmaf(s, a, 0.05614964838604722f);
-	s = __builtin_fmaf(s, a, -0.129972558952652f);
-	s = __builtin_fmaf(s, a, 0.24927933010348388f);
-	s = __builtin_fmaf(s, a, -0.7978181460806049f);
-	s = __builtin_fmaf(s, a, 0.49999899605353737f);
+	float s = -8.063526421414195e-06f;
+	s = __builtin_fmaf(s, a, 0.00015194949927050064f);
+	s = __builtin_fmaf(s, a, -0.0012712149702726438f);
+	s = __builtin_fmaf(s, a, 0.006383002906360614f);
+	s = __builtin_fmaf(s, a, -0.02223130768127502f);
+	s = __builtin_fmaf(s, a, 0.05949735447645309f);
+	s = __builtin_fmaf(s, a, -0.1317733057963848f);
+	s = __builtin_fmaf(s, a, 0.24975246260495018f);
+	s = __builtin_fmaf(s, a, -0.797864929825654f);
+	s = __builtin_fmaf(s, a, 0.49999974472528175f);
 	s *= bell;
 	return z < 0.0f ? s : 1.0f - s;  // the slopes at z and -z add up to 1
 }

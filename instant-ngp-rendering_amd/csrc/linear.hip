@@ -975,7 +975,8 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
 			const size_t each = (stages + splits - 1) / splits, used = (stages + each - 1) / each;
 			const double n = (double)((tiles * used + 255) / 256);
 			const double join = used > 1 ? 3.0 + 8e-6 * (double)used * (double)M * N / 4.2 : 0.0;
-			const double t = 4.0 + 0.4 * n + each * std::max(kind.least, kind.each * n) + join;
+			const double finish = 0.4 * (kind.tile / 64) * (kind.tile / 64);  // a tile's results at a CU's share of the memory's rate
+			const double t = 4.0 + finish * n + each * std::max(kind.least, kind.each * n) + join;
 			if (t >= best.us) continue;
 			best.us = t;
 			best.tile = kind.tile;
@@ -1015,8 +1016,10 @@ static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size
 	ProductArgs a{p, q, M, K, plan.k_each, N, plan.tiles_m, plan.tiles_n, plan.splits, nullptr};
 	if (plan.splits > 1) a.partial = room.take<float>((size_t)plan.splits * M * up8(N));
 	if (!room.run) return;
+	// (up to two stages of K take two buffers: more workgroups per CU hide what one stage cannot)
 	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, WIDE_THREADS, 131072, a, out, s);
 	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128, 2>, PRODUCT_THREADS, 2 * 32768, a, out, s);
+	else if (plan.k_each <= 2 * PRODUCT_K) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64, 2>, PRODUCT_THREADS, 2 * 16384, a, out, s);
 	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64, 3>, PRODUCT_THREADS, 3 * 16384, a, out, s);
 	if (plan.splits > 1) {
 		join<T>(a.partial, plan.splits, M, N, out, s);
@@ -1041,6 +1044,8 @@ static Matrix operand(const Kept<T>& v, int act, size_t rows, uint32_t width, Ro
 	}
 	return {to, up8(width)};
 }
+
+constexpr uint32_t NARROW_WIDTH = 128, NARROW_ROWS = 16384;
 
 template <class T>
 static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) {
@@ -1069,9 +1074,8 @@ static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) 
 	return room.bytes;
 }
 
-// Narrow layers in one pass, where there are rows enough for every CU's first turn: two workgroups per CU, for 128 x 128 (with
-// four times the sums to leave behind) one.
-constexpr uint32_t NARROW_WIDTH = 128, NARROW_ROWS = 16384;
+// Narrow layers' backward in one pass, where there are rows enough for every CU's first turn: two workgroups per CU, for
+// 128 x 128 (with four times the sums to leave behind) one.
 template <class T, int NI, int NO>
 static void launch_narrow(const NarrowArgs<T>& a, uint32_t grid, hipStream_t s) {
 	auto kernel = a.n_in % 8 == 0 && a.n_out % 8 == 0 ? k_narrow_backward<T, NI, NO, true> : k_narrow_backward<T, NI, NO, false>;

@@ -200,7 +200,17 @@ def test_backward(n, n_in, n_out, kind):
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("n, n_in, n_out", [(16384, 64, 64), (16385, 16, 16), (20011, 128, 128), (40001, 33, 67), (17000, 100, 64), (16500, 3, 120),
                                             (16999, 128, 8), (100003, 1, 1)])
-def test_backward_of_narrow_layers(n, n_in, n_out, kind):
+def test_narrow_layers(n, n_in, n_out, kind):
+    t = U.TYPES[kind][1]
+    for seed, name in enumerate(("relu", "gelu")):
+        x, w, b, r = normal(seed, n, n_in, t=t), normal(seed + 1, n_out, n_in, scale=n_in ** -0.5, t=t), normal(seed + 2, n_out), normal(seed + 3, n, n_out, t=t)
+        z, z8 = torch.empty(n, n_out, dtype=t, device="cuda"), U.new8(n, n_out)
+        y = U.call_linear(kind, x, w, b, name, r if seed else None, z=z, z8=z8 if seed else None)
+        ze, ztol, ye, ytol = forward_reference(x, w, b, name, r if seed else None)
+        close(y, ye, ytol + U.rounding(ye.abs() + ytol, t), name)
+        close(z, ze, ztol + U.rounding(ze.abs() + ztol, t), "z")
+        if seed:
+            check_checkpoint(z8, ze, ztol, kind)
     for seed, (name, x_name, z8, x8) in enumerate((("relu", "none", False, False), ("silu", "gelu", True, True), ("none", "relu", False, True))):
         dy, xk, zk, w, x, z = backward_inputs(kind, n, n_in, n_out, seed, z8, x8)
         every = U.call_linear_backward(kind, dy, xk, w, name, zk if name != "none" else None, x_name)
@@ -216,14 +226,18 @@ def test_backward_of_narrow_layers(n, n_in, n_out, kind):
     check_backward(kind, got, dy, x, z, w, name, x_name, "f32", base)
 
 
-def test_backward_of_narrow_layers_strides_and_frames():
+def test_narrow_layers_strides_and_frames():
     t, nan = torch.float16, float("nan")
     for n, n_in, n_out, pad, offset in ((16400, 64, 40, 8, 0), (16400, 72, 64, 3, 1), (17001, 45, 91, 0, 1)):
         dy, x, z, w, dx, dw = (U.Framed(*s, t, pad, offset, value=nan, init=normal(k, *s, scale=0.2)) for k, s in enumerate(
             ((n, n_out), (n, n_in), (n, n_out), (n_out, n_in), (n, n_in), (n_out, n_in))))
         got = U.call_linear_backward("f16", dy.t, x.t, w.t, "gelu", z.t, "silu", dx=dx.t, dw=dw.t)
         check_backward("f16", got, dy.t, x.t.double(), z.t.double(), w.t, "gelu", "silu")
-        for m in (dy, x, z, w, dx, dw):
+        y = U.Framed(n, n_out, t, pad, offset)
+        U.call_linear("f16", x.t, w.t, None, "silu", z.t, y=y.t)
+        ze, ztol, ye, ytol = forward_reference(x.t, w.t, None, "silu", z.t)
+        close(y.t, ye, ytol + U.rounding(ye.abs() + ytol, t))
+        for m in (dy, x, z, w, dx, dw, y):
             assert m.untouched_outside()
 
 
