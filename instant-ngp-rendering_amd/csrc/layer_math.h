@@ -207,9 +207,9 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 struct Walk {
 	size_t i, di;
 	uint32_t e, de, eighths;
-	__device__ __forceinline__ explicit Walk(uint32_t eighths) : eighths(eighths) {
-		const size_t t = (size_t)blockIdx.x * 256u + threadIdx.x;
-		const uint32_t step = gridDim.x * 256u;
+	__device__ __forceinline__ explicit Walk(uint32_t eighths, uint32_t block = blockIdx.x, uint32_t blocks = gridDim.x) : eighths(eighths) {
+		const size_t t = (size_t)block * 256u + threadIdx.x;
+		const uint32_t step = blocks * 256u;
 		i = t / eighths;
 		e = (uint32_t)(t % eighths);
 		di = step / eighths;
@@ -281,28 +281,34 @@ inline Kept<T> kept(const void* v, uint32_t stride, const ngp_checkpoint8& c) {
 	return Kept<T>{static_cast<const T*>(v), stride, c.q, c.scale, c.q_stride, c.scale_stride};
 }
 
-// put(j, the sum of part[0 .. shares)[j]) for j < columns, in a fixed order: 16 columns by 64 shares at a time, four reads on
-// their way; a wave's four shares meet by lane exchange, the 16 waves in LDS.
-template <class Put>
-__global__ void __launch_bounds__(1024) k_column_sums(const float* __restrict__ part, uint32_t shares, size_t columns, Put put) {
+// put(j, the sum of part[0 .. shares)[j]) for j < columns, in a fixed order: 16 columns per workgroup by as many shares at a
+// time as there are threads for, four reads on their way; a wave's four shares meet by lane exchange, the waves in LDS.
+template <int THREADS, class Put>
+__device__ __forceinline__ void column_sums(const float* __restrict__ part, uint32_t shares, size_t columns, const Put& put, uint32_t block) {
+	constexpr uint32_t LINES = THREADS / 16;
 	const uint32_t c = threadIdx.x % 16u, line = threadIdx.x / 16u;
-	const size_t j = (size_t)blockIdx.x * 16u + c;
+	const size_t j = (size_t)block * 16u + c;
 	float sum[4] = {};
 	if (j < columns)
-		for (uint32_t k = line; k < shares; k += 256u)
+		for (uint32_t k = line; k < shares; k += 4u * LINES)
 #pragma unroll
 			for (uint32_t u = 0; u < 4; ++u)
-				if (k + 64u * u < shares) sum[u] += part[(size_t)(k + 64u * u) * columns + j];
+				if (k + LINES * u < shares) sum[u] += part[(size_t)(k + LINES * u) * columns + j];
 	float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 	v += __shfl_xor(v, 16);
 	v += __shfl_xor(v, 32);
-	__shared__ float s[16][16];
+	__shared__ float s[THREADS / 64][16];
 	if (threadIdx.x % 64u < 16u) s[threadIdx.x / 64u][c] = v;
 	__syncthreads();
 	if (line || j >= columns) return;
 	v = 0.0f;
-	for (int w = 0; w < 16; ++w) v += s[w][c];
+	for (int w = 0; w < THREADS / 64; ++w) v += s[w][c];
 	put(j, v);
+}
+
+template <class Put>
+__global__ void __launch_bounds__(1024) k_column_sums(const float* __restrict__ part, uint32_t shares, size_t columns, Put put) {
+	column_sums<1024>(part, shares, columns, put, blockIdx.x);
 }
 
 template <class Put>

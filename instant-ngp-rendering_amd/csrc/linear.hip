@@ -295,9 +295,9 @@ template <int BM, int BN>
 struct Place {
 	uint32_t split, n0;
 	size_t m0, k0, k1;
-	__device__ __forceinline__ explicit Place(const ProductArgs& a) {
-		const uint32_t tiles = a.tiles_m * a.tiles_n, all = gridDim.x, xcd = blockIdx.x % 8u;
-		const uint32_t id = xcd * (all / 8u) + min(xcd, all % 8u) + blockIdx.x / 8u;
+	__device__ __forceinline__ Place(const ProductArgs& a, uint32_t block, uint32_t blocks) {
+		const uint32_t tiles = a.tiles_m * a.tiles_n, xcd = block % 8u;
+		const uint32_t id = xcd * (blocks / 8u) + min(xcd, blocks % 8u) + block / 8u;
 		split = id / tiles;
 		const uint32_t tile = id % tiles, group = tile / (8u * a.tiles_n), first = group * 8u, deep = min(8u, a.tiles_m - first);
 		const uint32_t in_group = tile - group * 8u * a.tiles_n;
@@ -404,15 +404,14 @@ __device__ __forceinline__ void meet() {
 // work on one stage, the others are on their way from memory into LDS without passing registers.  P's rows are the matrix
 // instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN, int BUFFERS>
-__global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, Out out) {
+__device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& out, uint32_t block, uint32_t blocks, char* lds) {
 	constexpr int TM = BM / 64, TN = BN / 64;  // 32 x 32 tiles per wave
 	typedef Stage<T, BM, P_BY_K, 64, PRODUCT_THREADS> PStage;
 	typedef Stage<T, BN, Q_BY_K, 64, PRODUCT_THREADS> QStage;
 	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
 	static_assert(4 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
-	extern __shared__ __attribute__((aligned(16))) char lds[];
 
-	const Place<BM, BN> at(a);
+	const Place<BM, BN> at(a, block, blocks);
 	const uint32_t wave = threadIdx.x / 64u;
 	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
 	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + 63u) / 64u);
@@ -470,6 +469,31 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, O
 	write_out(at.split, reinterpret_cast<float*>(lds) + wave * STRIP<TN>, c);
 }
 
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int TILE, int BUFFERS>
+__global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, Out out) {
+	extern __shared__ __attribute__((aligned(16))) char lds[];
+	product_tile<T, Out, P_BY_K, Q_BY_K, TILE, TILE, BUFFERS>(a, out, blockIdx.x, gridDim.x, lds);
+}
+
+// A layer's dx and dW, and the join of db's shares, side by side in one launch: none of them fills the GPU in layers whose
+// products take the smaller tiles, and none waits for another.
+struct Sums {
+	const float* part;
+	uint32_t shares, columns;
+	PutSums put;
+};
+template <class T, int TILE, int BUFFERS>
+__global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(ProductArgs dx, GradientOut<T> dx_out, uint32_t dx_blocks, ProductArgs dw,
+                                                                          WeightsOut<T> dw_out, uint32_t dw_blocks, Sums sums) {
+	extern __shared__ __attribute__((aligned(16))) char lds[];
+	if (blockIdx.x < dx_blocks)
+		product_tile<T, GradientOut<T>, false, true, TILE, TILE, BUFFERS>(dx, dx_out, blockIdx.x, dx_blocks, lds);
+	else if (blockIdx.x - dx_blocks < dw_blocks)
+		product_tile<T, WeightsOut<T>, true, true, TILE, TILE, BUFFERS>(dw, dw_out, blockIdx.x - dx_blocks, dw_blocks, lds);
+	else
+		column_sums<PRODUCT_THREADS>(sums.part, sums.shares, sums.columns, sums.put, blockIdx.x - dx_blocks - dw_blocks);
+}
+
 // 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
 // reads its next fragments and asks for a stage of K ahead, and then they change places.  A barrier after each half keeps
 // the two sets of four waves in opposite phases.  K goes through 128 KiB of LDS in stages of DEEP, each multiplied in steps
@@ -483,7 +507,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 	static_assert(8 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
 	extern __shared__ __attribute__((aligned(16))) char lds[];
 
-	const Place<BM, BN> at(a);
+	const Place<BM, BN> at(a, blockIdx.x, gridDim.x);
 	const uint32_t wave = threadIdx.x / 64u;
 	const uint32_t wm = wave / 4u * 128u, wn = wave % 4u * 64u;
 	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + DEEP - 1) / DEEP);
@@ -879,57 +903,87 @@ struct PutNarrow {
 };
 
 // ---- operands that do not lie as the product wants them ---------------------------------------------------------------
-// act(v), rounded to T, in rows of `width` up to 8, filled up with zeros.
-template <class T, bool VALUES>
-__global__ void __launch_bounds__(256) k_lay_out(Kept<T> v, int act, size_t rows, uint32_t width, T* __restrict__ to) {
-	const uint32_t w8 = (width + 7u) & ~7u;
-	for (Walk w(w8 / 8u); w.i < rows; w.next()) {
-		const uint32_t j = w.e * 8u;
-		float x[8];
-		v.template at8_of<VALUES>(w.i, j, width - j, x);
-		act_values(act, x);
-		if (width - j < 8u)
-#pragma unroll
-			for (int k = 0; k < 8; ++k) x[k] = j + k < width ? x[k] : 0.0f;
-		store8(to + w.i * w8 + j, 8, x);
-	}
-}
-
-// dz = dy act'(z), in rows of `width` up to 8 (dz null: not kept), and its sums over a share of the rows.  A workgroup
-// takes 8 * groups columns (groups a power of two up to 32) and 256 / groups rows at a time.
+// act(v), rounded to T, in rows of `width` up to 8, filled up with zeros, by `blocks` workgroups.
 template <class T>
-__global__ void __launch_bounds__(256) k_linear_dz(Kept<T> dy, Kept<T> z, int act, size_t n, uint32_t width, uint32_t groups,
-                                                   size_t rows_each, T* __restrict__ dz, float* __restrict__ part) {
-	const uint32_t g = threadIdx.x % groups, lines = 256u / groups, j = (blockIdx.x * groups + g) * 8u;
-	const size_t begin = blockIdx.y * rows_each, end = min(begin + rows_each, n);
-	const uint32_t w8 = (width + 7u) & ~7u;
-	float sum[8] = {};
-	if (j < width)
-		for (size_t i = begin + threadIdx.x / groups; i < end; i += lines) {
-			float d[8];
-			dy.at8(i, j, width - j, d);
-			if (act != NGP_ACT_NONE) {
-				float s[8];
-				z.at8(i, j, width - j, s);
-				act_slopes(act, s);
+struct LayOut {
+	Kept<T> v;
+	int act = NGP_ACT_NONE;
+	size_t rows = 0;
+	uint32_t width = 0, blocks = 0;
+	T* to = nullptr;
+	template <bool VALUES>
+	__device__ __forceinline__ void run(uint32_t block) const {
+		const uint32_t w8 = (width + 7u) & ~7u;
+		for (Walk w(w8 / 8u, block, blocks); w.i < rows; w.next()) {
+			const uint32_t j = w.e * 8u;
+			float x[8];
+			v.template at8_of<VALUES>(w.i, j, width - j, x);
+			act_values(act, x);
+			if (width - j < 8u)
 #pragma unroll
-				for (int k = 0; k < 8; ++k) d[k] = j + k < width ? d[k] * s[k] : 0.0f;
-			}
-			if (dz) store8(dz + i * w8 + j, 8, d);
-#pragma unroll
-			for (int k = 0; k < 8; ++k) sum[k] += d[k];
+				for (int k = 0; k < 8; ++k) x[k] = j + k < width ? x[k] : 0.0f;
+			store8(to + w.i * w8 + j, 8, x);
 		}
-	if (!part) return;
-	__shared__ float s[256][9];
+	}
+};
+
+// dz = dy act'(z), in rows of `width` up to 8 (to null: not kept), and its sums over a share of the rows (part null: not
+// wanted).  A workgroup takes 8 * groups columns (groups a power of two up to 32) and 256 / groups rows at a time; `wide`
+// workgroups lie side by side.
+template <class T>
+struct MakeDz {
+	Kept<T> dy, z;
+	int act = NGP_ACT_NONE;
+	size_t n = 0, rows_each = 0;
+	uint32_t width = 0, groups = 1, wide = 1, blocks = 0;
+	T* to = nullptr;
+	float* part = nullptr;
+	__device__ __forceinline__ void run(uint32_t block) const {
+		const uint32_t side = block % wide, share = block / wide;
+		const uint32_t g = threadIdx.x % groups, lines = 256u / groups, j = (side * groups + g) * 8u;
+		const size_t begin = share * rows_each, end = min(begin + rows_each, n);
+		const uint32_t w8 = (width + 7u) & ~7u;
+		float sum[8] = {};
+		if (j < width)
+			for (size_t i = begin + threadIdx.x / groups; i < end; i += lines) {
+				float d[8];
+				dy.template at8_of<true>(i, j, width - j, d);
+				if (act != NGP_ACT_NONE) {
+					float s[8];
+					z.at8(i, j, width - j, s);
+					act_slopes(act, s);
 #pragma unroll
-	for (int k = 0; k < 8; ++k) s[threadIdx.x][k] = sum[k];
-	__syncthreads();
-	if (threadIdx.x >= groups * 8u) return;
-	const uint32_t column = blockIdx.x * groups * 8u + threadIdx.x;
-	if (column >= width) return;
-	float total = 0.0f;
-	for (uint32_t l = 0; l < lines; ++l) total += s[l * groups + threadIdx.x / 8u][threadIdx.x % 8u];
-	part[(size_t)blockIdx.y * width + column] = total;
+					for (int k = 0; k < 8; ++k) d[k] = j + k < width ? d[k] * s[k] : 0.0f;
+				}
+				if (to) store8(to + i * w8 + j, 8, d);
+#pragma unroll
+				for (int k = 0; k < 8; ++k) sum[k] += d[k];
+			}
+		if (!part) return;
+		__shared__ float s[256][9];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) s[threadIdx.x][k] = sum[k];
+		__syncthreads();
+		if (threadIdx.x >= groups * 8u) return;
+		const uint32_t column = side * groups * 8u + threadIdx.x;
+		if (column >= width) return;
+		float total = 0.0f;
+		for (uint32_t l = 0; l < lines; ++l) total += s[l * groups + threadIdx.x / 8u][threadIdx.x % 8u];
+		part[(size_t)share * width + column] = total;
+	}
+};
+
+// What the products need first, side by side in one launch.
+template <class T>
+__global__ void __launch_bounds__(256) k_prepare(MakeDz<T> dz, LayOut<T> a, LayOut<T> b) {
+	if (blockIdx.x < dz.blocks) {
+		dz.run(blockIdx.x);
+		return;
+	}
+	const bool first = blockIdx.x - dz.blocks < a.blocks;
+	const LayOut<T>& l = first ? a : b;
+	const uint32_t block = blockIdx.x - dz.blocks - (first ? 0u : a.blocks);
+	l.v.v ? l.template run<true>(block) : l.template run<false>(block);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -962,7 +1016,7 @@ struct ProductPlan {
 // (1024^3: 8 us with 64 tiles, 12 with 128, 25 with 256), a 256 tile moves a quarter of the bytes per multiplication (4096 x
 // 2048 x 4096: 105, 70 and 60 us).  Splits write their sums and read them again at about 4.2 TB/s, in a launch of their own
 // (32 x 4096 x 4096: 19 us with 64 tiles, 12 with four splits; 2048 x 1024 x 1024: 10 us, 24 with two).
-static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
+static ProductPlan plan_product(size_t M, uint32_t N, size_t K, int only = 0) {
 	struct Kind {
 		int tile;
 		double least, each;
@@ -970,6 +1024,7 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K) {
 	ProductPlan best;
 	const size_t stages = std::max<size_t>(1, (K + PRODUCT_K - 1) / PRODUCT_K);
 	for (const Kind& kind : {Kind{64, 0.23, 0.185}, Kind{128, 0.5, 0.52}, Kind{256, 1.3, 1.68}}) {
+		if (only && kind.tile != only) continue;
 		const size_t tiles = ((M + kind.tile - 1) / kind.tile) * (((size_t)N + kind.tile - 1) / kind.tile);
 		for (size_t splits = 1; splits <= std::min<size_t>(64, stages); splits *= 2) {
 			const size_t each = (stages + splits - 1) / splits, used = (stages + each - 1) / each;
@@ -1008,22 +1063,22 @@ static void join(const float* partial, uint32_t splits, size_t M, uint32_t N, co
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
-// C[M][N] = P Q^T to `out`; a Room that does not run only counts what it takes.
-template <class T, class Out, bool P_BY_K, bool Q_BY_K>
-static void product(const Matrix& p, const Matrix& q, size_t M, uint32_t N, size_t K, const Out& out, Room& room, hipStream_t s) {
-	if (!M) return;
-	const ProductPlan plan = plan_product(M, N, K);
+// C[M][N] = P Q^T by a plan; the splits' sums take their place in the workspace.
+static ProductArgs product_args(const ProductPlan& plan, const Matrix& p, const Matrix& q, size_t M, uint32_t N, size_t K, Room& room) {
 	ProductArgs a{p, q, M, K, plan.k_each, N, plan.tiles_m, plan.tiles_n, plan.splits, nullptr};
 	if (plan.splits > 1) a.partial = room.take<float>((size_t)plan.splits * M * up8(N));
-	if (!room.run) return;
-	// (up to two stages of K take two buffers: more workgroups per CU hide what one stage cannot)
+	return a;
+}
+// (up to two stages of K take two buffers: more workgroups per CU hide what one stage cannot)
+static bool is_short(const ProductPlan& plan) { return plan.k_each <= 2 * PRODUCT_K; }
+
+template <class T, class Out, bool P_BY_K, bool Q_BY_K>
+static void product(const ProductPlan& plan, const ProductArgs& a, const Out& out, hipStream_t s) {
 	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, WIDE_THREADS, 131072, a, out, s);
-	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 128, 2>, PRODUCT_THREADS, 2 * 32768, a, out, s);
-	else if (plan.k_each <= 2 * PRODUCT_K) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64, 2>, PRODUCT_THREADS, 2 * 16384, a, out, s);
-	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 64, 3>, PRODUCT_THREADS, 3 * 16384, a, out, s);
-	if (plan.splits > 1) {
-		join<T>(a.partial, plan.splits, M, N, out, s);
-	}
+	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 2>, PRODUCT_THREADS, 2 * 32768, a, out, s);
+	else if (is_short(plan)) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 2>, PRODUCT_THREADS, 2 * 16384, a, out, s);
+	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 3>, PRODUCT_THREADS, 3 * 16384, a, out, s);
+	if (a.splits > 1) join<T>(a.partial, a.splits, a.M, a.N, out, s);
 }
 
 // Whether a product's loads, 16 bytes at a time, can take a matrix where it lies.
@@ -1031,18 +1086,22 @@ static bool in_place(const void* p, size_t stride, uint32_t width) {
 	return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && width % 8 == 0;
 }
 
-// `v` where it lies if the product can read it there, else act(v) copied to the workspace.
+// `v` where it lies if the product can read it there, else act(v) copied to the workspace by `lay`.
 template <class T>
-static Matrix operand(const Kept<T>& v, int act, size_t rows, uint32_t width, Room& room, hipStream_t s) {
+static Matrix operand(const Kept<T>& v, int act, size_t rows, uint32_t width, Room& room, LayOut<T>& lay) {
 	if (v.v && act == NGP_ACT_NONE && in_place(v.v, v.stride, width)) return {v.v, v.stride};
 	T* to = room.take<T>(rows * up8(width));
-	if (room.run && rows) {
-		const size_t blocks = (rows * (up8(width) / 8) + 255) / 256;
-		auto kernel = v.v ? k_lay_out<T, true> : k_lay_out<T, false>;
-		kernel<<<(uint32_t)std::min<size_t>(blocks, 16384), 256, 0, s>>>(v, act, rows, width, to);
-		NGP_HIP_CHECK(hipGetLastError());
-	}
+	const size_t blocks = (rows * (up8(width) / 8) + 255) / 256;
+	lay = LayOut<T>{v, act, rows, width, (uint32_t)std::min<size_t>(blocks, 16384), to};
 	return {to, up8(width)};
+}
+
+template <class T>
+static void prepare(const MakeDz<T>& dz, const LayOut<T>& a, const LayOut<T>& b, hipStream_t s) {
+	const uint32_t blocks = dz.blocks + a.blocks + b.blocks;
+	if (!blocks) return;
+	k_prepare<T><<<blocks, 256, 0, s>>>(dz, a, b);
+	NGP_HIP_CHECK(hipGetLastError());
 }
 
 constexpr uint32_t NARROW_WIDTH = 128, NARROW_ROWS = 16384;
@@ -1068,9 +1127,14 @@ static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) 
 		NGP_HIP_CHECK(hipGetLastError());
 		return 0;
 	}
-	const Matrix x = operand<T>(kept<T>(a.x, a.x_stride, {}), NGP_ACT_NONE, a.n, a.n_in, room, s);
-	const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
-	product<T, ForwardOut<T>, false, false>(x, w, a.n, a.n_out, a.n_in, out, room, s);
+	LayOut<T> lay_x, lay_w;
+	const Matrix x = operand<T>(kept<T>(a.x, a.x_stride, {}), NGP_ACT_NONE, a.n, a.n_in, room, lay_x);
+	const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, lay_w);
+	const ProductPlan plan = plan_product(a.n, a.n_out, a.n_in);
+	const ProductArgs args = product_args(plan, x, w, a.n, a.n_out, a.n_in, room);
+	if (!run) return room.bytes;
+	prepare<T>({}, lay_x, lay_w, s);
+	product<T, ForwardOut<T>, false, false>(plan, args, out, s);
 	return room.bytes;
 }
 
@@ -1107,38 +1171,68 @@ template <class T>
 static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipStream_t s) {
 	if (a.n >= NARROW_ROWS && a.n_in <= NARROW_WIDTH && a.n_out <= NARROW_WIDTH && (a.dx || a.dweights)) return narrow_backward<T>(a, run, s);
 	Room room{static_cast<char*>(a.workspace), run};
-	const bool products = a.dx || a.dweights, active = a.activation != NGP_ACT_NONE;
-	const Kept<T> dy = kept<T>(a.dy, a.dy_stride, {}), x = kept<T>(a.x, a.x_stride, a.x8);
+	const bool want_dx = a.dx && a.n, want_dw = a.dweights;
+	const Kept<T> x = kept<T>(a.x, a.x_stride, a.x8);
 	// dz where it has to be made, or copied into rows that the products can read
-	const bool make_dz = products && (active || !in_place(a.dy, a.dy_stride, a.n_out));
+	const bool make_dz = (want_dx || want_dw) && (a.activation != NGP_ACT_NONE || !in_place(a.dy, a.dy_stride, a.n_out));
 	T* dz_to = make_dz ? room.take<T>((size_t)a.n * up8(a.n_out)) : nullptr;
 	const Matrix dz = make_dz ? Matrix{dz_to, up8(a.n_out)} : Matrix{a.dy, a.dy_stride};
+	MakeDz<T> job;
+	Sums sums{nullptr, 0, 0, {a.dbias, nullptr, a.n_out, a.accumulate != 0}};
 	if (make_dz || a.dbias) {
-		// every workgroup takes 32 rows at least; about four workgroups per CU
 		uint32_t groups = 1;
 		while (groups < 32 && groups * 8 < a.n_out) groups *= 2;
 		const uint32_t wide = (a.n_out + groups * 8 - 1) / (groups * 8), lines = 256 / groups;
-		const uint32_t shares = (uint32_t)std::max<size_t>(1, std::min<size_t>((a.n + lines - 1) / lines, std::max(1u, 1024u / wide)));
-		const size_t each = ((size_t)a.n + shares - 1) / shares;
+		// about four workgroups per CU
+		const uint32_t shares = (uint32_t)std::max<size_t>(1, std::min<size_t>(((size_t)a.n + lines - 1) / lines, std::max(1u, 1024u / wide)));
 		float* part = a.dbias ? room.take<float>((size_t)shares * a.n_out) : nullptr;
-		if (run) {
-			k_linear_dz<T><<<dim3(wide, shares), 256, 0, s>>>(dy, kept<T>(a.z, a.z_stride, a.z8), a.activation, a.n, a.n_out, groups, each,
-			                                                 dz_to, part);
-			NGP_HIP_CHECK(hipGetLastError());
-			if (a.dbias) launch_column_sums(part, shares, a.n_out, PutSums{a.dbias, nullptr, a.n_out, a.accumulate != 0}, s);
-		}
+		job = MakeDz<T>{kept<T>(a.dy, a.dy_stride, {}), kept<T>(a.z, a.z_stride, a.z8), a.activation, a.n, ((size_t)a.n + shares - 1) / shares,
+		                a.n_out, groups, wide, wide * shares, dz_to, part};
+		if (a.dbias) sums.part = part, sums.shares = shares, sums.columns = a.n_out;
 	}
-	if (a.dx && a.n) {
-		const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, s);
-		const GradientOut<T> out{static_cast<T*>(a.dx), a.dx_stride, x, a.x_activation};
-		product<T, GradientOut<T>, false, true>(dz, w, a.n, a.n_in, a.n_out, out, room, s);
+	LayOut<T> lay_w, lay_x;
+	ProductPlan dx_plan, dw_plan;
+	ProductArgs dx_args{}, dw_args{};
+	if (want_dx) dx_plan = plan_product(a.n, a.n_in, a.n_out);
+	if (want_dw) dw_plan = plan_product(a.n_out, a.n_in, a.n);
+	bool together = want_dx && want_dw && dx_plan.tile < 256 && dw_plan.tile < 256;
+	if (together && dx_plan.tile != dw_plan.tile) {  // side by side they need the same tile
+		const ProductPlan dx64 = plan_product(a.n, a.n_in, a.n_out, 64), dx128 = plan_product(a.n, a.n_in, a.n_out, 128);
+		const ProductPlan dw64 = plan_product(a.n_out, a.n_in, a.n, 64), dw128 = plan_product(a.n_out, a.n_in, a.n, 128);
+		const bool small = dx64.us + dw64.us < dx128.us + dw128.us;
+		dx_plan = small ? dx64 : dx128;
+		dw_plan = small ? dw64 : dw128;
 	}
-	if (a.dweights) {
-		const Matrix xs = operand<T>(x, a.x_activation, a.n, a.n_in, room, s);
-		const bool f32 = a.dweights_type == NGP_TYPE_F32;
-		const WeightsOut<T> out{a.dweights, a.dweights_stride, f32, a.accumulate != 0};
-		product<T, WeightsOut<T>, true, true>(dz, xs, a.n_out, a.n_in, a.n, out, room, s);
+	if (want_dx) {
+		const Matrix w = operand<T>(kept<T>(a.weights, a.weights_stride, {}), NGP_ACT_NONE, a.n_out, a.n_in, room, lay_w);
+		dx_args = product_args(dx_plan, dz, w, a.n, a.n_in, a.n_out, room);
 	}
+	if (want_dw) {
+		const Matrix xs = operand<T>(x, a.x_activation, a.n, a.n_in, room, lay_x);
+		dw_args = product_args(dw_plan, dz, xs, a.n_out, a.n_in, a.n, room);
+	}
+	if (!run) return room.bytes;
+
+	prepare<T>(job, lay_w, lay_x, s);
+	const GradientOut<T> dx_out{static_cast<T*>(a.dx), a.dx_stride, x, a.x_activation};
+	const WeightsOut<T> dw_out{a.dweights, a.dweights_stride, a.dweights_type == NGP_TYPE_F32, a.accumulate != 0};
+	if (together) {
+		const uint32_t dx_blocks = dx_args.tiles_m * dx_args.tiles_n * dx_args.splits, dw_blocks = dw_args.tiles_m * dw_args.tiles_n * dw_args.splits;
+		const uint32_t blocks = dx_blocks + dw_blocks + (sums.columns + 15) / 16;
+		if (dx_plan.tile == 128)
+			k_backward_products<T, 128, 2><<<blocks, PRODUCT_THREADS, 2 * 32768, s>>>(dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
+		else if (is_short(dx_plan) && is_short(dw_plan))
+			k_backward_products<T, 64, 2><<<blocks, PRODUCT_THREADS, 2 * 16384, s>>>(dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
+		else
+			k_backward_products<T, 64, 3><<<blocks, PRODUCT_THREADS, 3 * 16384, s>>>(dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
+		NGP_HIP_CHECK(hipGetLastError());
+		if (dx_args.splits > 1) join<T>(dx_args.partial, dx_args.splits, a.n, a.n_in, dx_out, s);
+		if (dw_args.splits > 1) join<T>(dw_args.partial, dw_args.splits, a.n_out, a.n_in, dw_out, s);
+		return room.bytes;
+	}
+	if (sums.columns) launch_column_sums(sums.part, sums.shares, sums.columns, sums.put, s);
+	if (want_dx) product<T, GradientOut<T>, false, true>(dx_plan, dx_args, dx_out, s);
+	if (want_dw) product<T, WeightsOut<T>, true, true>(dw_plan, dw_args, dw_out, s);
 	return room.bytes;
 }
 
