@@ -553,7 +553,7 @@ ngp_status ngp_accumulate_tonemap(const float* frame, float* accum, float* out, 
  * activations a backward pass needs kept in 8 bits.  No model handle: every call works on the caller's device memory on
  * `stream` (of the current device, or of the stream's own device), allocates nothing, never waits for the device and
  * may be captured into a graph; what a call reads and writes must live until the stream has passed it.
- *  - Matrices are row-major, strides in elements, at least the width and below 2^22; widths are 1..65536, rows 0..2^31-1.
+ *  - Matrices are row-major, strides in elements, at least the width and below 2^22; widths are 1..65536, rows 0..2^29.
  *    Rows that start on 16 bytes (16-byte aligned pointers, strides that are multiples of 8 elements) and widths that are
  *    multiples of 8 run in place; other layers' matrices are first copied into the workspace.
  *  - Outputs must not overlap inputs or each other, except: y may be residual, dx may be dx_add (the same rows).

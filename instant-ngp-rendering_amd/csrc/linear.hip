@@ -1026,8 +1026,10 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K, int only = 0) {
 	for (const Kind& kind : {Kind{64, 0.23, 0.185}, Kind{128, 0.5, 0.52}, Kind{256, 1.3, 1.68}}) {
 		if (only && kind.tile != only) continue;
 		const size_t tiles = ((M + kind.tile - 1) / kind.tile) * (((size_t)N + kind.tile - 1) / kind.tile);
+		if (tiles >= 1u << 23) continue;  // (a launch has fewer than 2^32 threads; 256 tiles hold every matrix that memory does)
 		for (size_t splits = 1; splits <= std::min<size_t>(64, stages); splits *= 2) {
 			const size_t each = (stages + splits - 1) / splits, used = (stages + each - 1) / each;
+			if (used > 1 && tiles * used > 65536) break;
 			const double n = (double)((tiles * used + 255) / 256);
 			const double join = used > 1 ? 3.0 + 8e-6 * (double)used * (double)M * N / 4.2 : 0.0;
 			const double finish = 0.4 * (kind.tile / 64) * (kind.tile / 64);  // a tile's results at a CU's share of the memory's rate

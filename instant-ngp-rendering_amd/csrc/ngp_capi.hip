@@ -818,7 +818,7 @@ struct OnDeviceOf {
 };
 }  // namespace
 
-constexpr uint32_t LAYER_WIDTH_MAX = 65536, LAYER_STRIDE_END = 1u << 22, LAYER_ROWS_MAX = 0x7fffffffu;
+constexpr uint32_t LAYER_WIDTH_MAX = 65536, LAYER_STRIDE_END = 1u << 22, LAYER_ROWS_MAX = 1u << 29;
 
 static size_t type_size(int type) { return type == NGP_TYPE_F32 ? 4 : 2; }
 static void require_type(int type) {
@@ -831,7 +831,7 @@ static void require_act(int act) { require(act >= 0 && act < NGP_ACT_COUNT, "act
 static void require_width(uint32_t width) {
 	require(width >= 1 && width <= LAYER_WIDTH_MAX, "widths must be in [1, 65536]");
 }
-static void require_rows(uint32_t n) { require(n <= LAYER_ROWS_MAX, "at most 2^31 - 1 rows"); }
+static void require_rows(uint32_t n) { require(n <= LAYER_ROWS_MAX, "at most 2^29 rows"); }
 // a matrix that is there: aligned to its elements, a stride that holds its rows
 static void require_matrix(const void* p, uint32_t stride, uint32_t width, size_t element) {
 	if (!p) return;

@@ -490,8 +490,9 @@ def test_a_residual_block_learns_what_its_formula_says(kind, n, d, hidden):
         assert err < (5 * U.half_step(U.TYPES[kind][1]) if k == "y" else 0.04), (k, float(err))
 
 
-def test_the_same_result_every_time_on_any_stream_and_in_graphs():
-    s = block_state("f16", 3000, 256, 512)
+@pytest.mark.parametrize("n, d, hidden", [(3000, 256, 512), (4200, 520, 4400), (20000, 64, 128), (9, 130, 200)])
+def test_the_same_result_every_time_on_any_stream_and_in_graphs(n, d, hidden):
+    s = block_state("f16", n, d, hidden)
     want = {k: v.clone() for k, v in residual_block("f16", s).items()}
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -503,7 +504,7 @@ def test_the_same_result_every_time_on_any_stream_and_in_graphs():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         held = residual_block_without_checks("f16", s)
-    fresh = block_state("f16", 3000, 256, 512, seed=50)
+    fresh = block_state("f16", n, d, hidden, seed=50)
     old = {k: v.clone() for k, v in s.items()}
     for step in range(4):
         source = old if step % 2 else fresh
@@ -529,6 +530,29 @@ def residual_block_without_checks(kind, s):
         return residual_block(kind, s), held
     finally:
         U.guards_hold = asked
+
+
+def test_many_rows():
+    n = 1 << 27  # more rows of a few values than a launch's threads
+    x = torch.full((n, 5), 2.0, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = -2.0
+    row = x[:1].double()
+    want, _, _ = U.layer_norm(row, torch.ones(5, device="cuda").double(), 0.0, 1e-5)
+    y, mean, rstd = U.call_layer_norm("bf16", x)
+    for i in (0, n // 2 + 1, n - 1):
+        close(y[i:i + 1], want, U.rounding(want, torch.bfloat16) * 1.01 + 1e-5)
+    assert torch.equal(y.amin(0), y.amax(0))
+    dx, dg, db = U.call_layer_norm_backward("bf16", x, x, mean, rstd, dx=y)
+    assert torch.equal(dx.amin(0), dx.amax(0))
+    # 2^27 equal terms: sums of 2^27 / 2^14 = 2^13 at most by one thread, then of their sums, each within half a step
+    close(dg, n * (row * want)[0], 2.0 ** -10 * n * (row * want)[0].abs() + 1)
+    close(db, n * row[0], 2.0 ** -10 * n * row[0].abs() + 1)
+    w = normal(1, 3, 5, t=torch.bfloat16)
+    out = U.call_linear("bf16", x, w)
+    close(out[n - 1:], row @ w.double().t(), U.rounding(row @ w.double().t(), torch.bfloat16) * 1.01 + 1e-5)
+    assert torch.equal(out.amin(0), out.amax(0))
+    c8 = U.call_store("bf16", x)
+    assert torch.equal(U.call_load("bf16", c8, 5, y), x)
 
 
 def test_offsets_past_32_bits():

@@ -56,7 +56,7 @@ EIGHT = A.Checkpoint8(HERE * 6, HERE * 7, 64, 2)
 
 @pytest.mark.parametrize("kw, text", [
     (dict(type=A.TYPE_F32), "NGP_TYPE_F16"), (dict(type=9), "NGP_TYPE_F16"), (dict(activation=6), "NGP_ACT"),
-    (dict(activation=-1), "NGP_ACT"), (dict(n=1 << 31), "rows"), (dict(n_in=0), "widths"), (dict(n_out=0), "widths"),
+    (dict(activation=-1), "NGP_ACT"), (dict(n=(1 << 29) + 1), "rows"), (dict(n_in=0), "widths"), (dict(n_out=0), "widths"),
     (dict(n_in=65537), "widths"), (dict(x=None), "null"), (dict(weights=None), "null"), (dict(y=None), "null"),
     (dict(x=HERE + 1), "aligned"), (dict(x_stride=7), "stride"), (dict(weights_stride=1 << 22), "stride"),
     (dict(y_stride=15), "stride"), (dict(residual=HERE * 9, residual_stride=3), "stride"),
@@ -75,7 +75,7 @@ def test_linear_refuses(kw, text):
 
 @pytest.mark.parametrize("kw, text", [
     (dict(type=A.TYPE_F32), "NGP_TYPE_F16"), (dict(activation=6), "NGP_ACT"), (dict(x_activation=-1), "NGP_ACT"),
-    (dict(n=1 << 31), "rows"), (dict(n_in=0), "widths"), (dict(n_out=1 << 20), "widths"), (dict(accumulate=2), "accumulate"),
+    (dict(n=(1 << 29) + 1), "rows"), (dict(n_in=0), "widths"), (dict(n_out=1 << 20), "widths"), (dict(accumulate=2), "accumulate"),
     (dict(dweights_type=A.TYPE_BF16), "dweights_type"), (dict(accumulate=1), "NGP_TYPE_F32 only"), (dict(dy=None), "null"),
     (dict(activation=A.ACT_GELU), "needs z or z8"), (dict(x=None), "needs x or x8"), (dict(weights=None), "needs the weights"),
     (dict(x=None, dweights=None, x_activation=A.ACT_RELU), "needs x or x8"), (dict(x8=EIGHT), "not in both"),
@@ -91,7 +91,7 @@ def test_linear_backward_refuses(kw, text):
 
 
 @pytest.mark.parametrize("kw, text", [
-    (dict(type=3), "NGP_TYPE"), (dict(n=1 << 31), "rows"), (dict(width=0), "widths"), (dict(width=65537), "widths"),
+    (dict(type=3), "NGP_TYPE"), (dict(n=(1 << 29) + 1), "rows"), (dict(width=0), "widths"), (dict(width=65537), "widths"),
     (dict(x=None), "null"), (dict(y=None), "null"), (dict(epsilon=-1.0), "epsilon"), (dict(epsilon=float("nan")), "epsilon"),
     (dict(x=HERE + 2), "aligned"), (dict(x_stride=39), "stride"), (dict(y_stride=1 << 22), "stride"),
     (dict(gamma=HERE + 1), "aligned"), (dict(mean=HERE + 2), "aligned"), (dict(y=HERE), "must not be"),
@@ -116,7 +116,7 @@ def test_layer_norm_backward_refuses(kw, text):
 
 @pytest.mark.parametrize("values, stride, n, width, kind, c, text", [
     (HERE, 40, 4, 40, 3, A.Checkpoint8(HERE, HERE, 40, 2), "NGP_TYPE"),
-    (HERE, 40, 1 << 31, 40, 0, A.Checkpoint8(HERE, HERE, 40, 2), "rows"),
+    (HERE, 40, (1 << 29) + 1, 40, 0, A.Checkpoint8(HERE, HERE, 40, 2), "rows"),
     (HERE, 40, 4, 0, 0, A.Checkpoint8(HERE, HERE, 40, 2), "widths"),
     (None, 40, 4, 40, 0, A.Checkpoint8(HERE, HERE, 40, 2), "null"),
     (HERE, 40, 4, 40, 0, A.Checkpoint8(None, None, 40, 2), "null"),
