@@ -403,26 +403,26 @@ __device__ __forceinline__ void meet() {
 // BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through BUFFERS LDS buffers: while the matrix cores
 // work on one stage, the others are on their way from memory into LDS without passing registers.  P's rows are the matrix
 // instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
-template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN, int BUFFERS>
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN, int DEEP, int BUFFERS>
 __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& out, uint32_t block, uint32_t blocks, char* lds) {
 	constexpr int TM = BM / 64, TN = BN / 64;  // 32 x 32 tiles per wave
-	typedef Stage<T, BM, P_BY_K, 64, PRODUCT_THREADS> PStage;
-	typedef Stage<T, BN, Q_BY_K, 64, PRODUCT_THREADS> QStage;
+	typedef Stage<T, BM, P_BY_K, DEEP, PRODUCT_THREADS> PStage;
+	typedef Stage<T, BN, Q_BY_K, DEEP, PRODUCT_THREADS> QStage;
 	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
 	static_assert(4 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
 
 	const Place<BM, BN> at(a, block, blocks);
 	const uint32_t wave = threadIdx.x / 64u;
 	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
-	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + 63u) / 64u);
+	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + DEEP - 1) / DEEP);
 
 	WriteOut<T, Out, TM, TN> write_out(a, out, at.m0 + wm, at.n0 + wn);
 	f32x16 c[TN][TM] = {};
 	if (stages) {
 		PStage ps;
 		QStage qs;
-		Fragments<PStage, BM, P_BY_K, 64, TM> pf;
-		Fragments<QStage, BN, Q_BY_K, 64, TN> qf;
+		Fragments<PStage, BM, P_BY_K, DEEP, TM> pf;
+		Fragments<QStage, BN, Q_BY_K, DEEP, TN> qf;
 		ps.begin(a.p, at.m0, a.M, at.k0, a.K);
 		qs.begin(a.q, at.n0, a.N, at.k0, a.K);
 		pf.begin(wm);
@@ -435,7 +435,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& ou
 			to = next(to);
 		};
 		// the part of K that fills no stage comes first, so that the loop has whole stages only
-		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % 64u) + 1u;
+		const uint32_t k_in = (uint32_t)((at.k1 - at.k0 - 1) % DEEP) + 1u;
 		ps.load_first(lds, k_in);
 		qs.load_first(lds + PStage::BYTES, k_in);
 		to = next(to);
@@ -455,8 +455,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& ou
 			};
 			read(0);
 #pragma unroll
-			for (int k = 0; k < 4; ++k) {
-				if (k < 3) read(k + 1);
+			for (int k = 0; k < DEEP / 16; ++k) {
+				if (k < DEEP / 16 - 1) read(k + 1);
 #pragma unroll
 				for (int n = 0; n < TN; ++n)
 #pragma unroll
@@ -472,7 +472,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& ou
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int TILE, int BUFFERS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, Out out) {
 	extern __shared__ __attribute__((aligned(16))) char lds[];
-	product_tile<T, Out, P_BY_K, Q_BY_K, TILE, TILE, BUFFERS>(a, out, blockIdx.x, gridDim.x, lds);
+	product_tile<T, Out, P_BY_K, Q_BY_K, TILE, TILE, 64, BUFFERS>(a, out, blockIdx.x, gridDim.x, lds);
 }
 
 // A layer's dx and dW, and the join of db's shares, side by side in one launch: none of them fills the GPU in layers whose
@@ -487,9 +487,9 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(Produc
                                                                           WeightsOut<T> dw_out, uint32_t dw_blocks, Sums sums) {
 	extern __shared__ __attribute__((aligned(16))) char lds[];
 	if (blockIdx.x < dx_blocks)
-		product_tile<T, GradientOut<T>, false, true, TILE, TILE, BUFFERS>(dx, dx_out, blockIdx.x, dx_blocks, lds);
+		product_tile<T, GradientOut<T>, false, true, TILE, TILE, 64, BUFFERS>(dx, dx_out, blockIdx.x, dx_blocks, lds);
 	else if (blockIdx.x - dx_blocks < dw_blocks)
-		product_tile<T, WeightsOut<T>, true, true, TILE, TILE, BUFFERS>(dw, dw_out, blockIdx.x - dx_blocks, dw_blocks, lds);
+		product_tile<T, WeightsOut<T>, true, true, TILE, TILE, 64, BUFFERS>(dw, dw_out, blockIdx.x - dx_blocks, dw_blocks, lds);
 	else
 		column_sums<PRODUCT_THREADS>(sums.part, sums.shares, sums.columns, sums.put, blockIdx.x - dx_blocks - dw_blocks);
 }
