@@ -522,6 +522,35 @@ def test_the_same_result_every_time_on_any_stream_and_in_graphs(n, d, hidden):
                 assert torch.equal(eager[k], want[k])
 
 
+def test_two_streams_at_once():
+    states = [block_state("bf16", n, d, hidden, seed) for n, d, hidden, seed in ((5000, 256, 1024, 0), (4000, 264, 1000, 40))]
+    want = [{k: v.clone() for k, v in residual_block("bf16", s).items()} for s in states]
+    streams = [torch.cuda.Stream() for _ in states]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, stream in zip(states, streams):  # nothing waits in between; every call has a workspace of its own
+            with torch.cuda.stream(stream):
+                got.append(residual_block_without_checks("bf16", s))
+        torch.cuda.synchronize()
+        for (out, rooms), w in zip(got, want):
+            assert all(U.guards_hold(r) for r in rooms)
+            assert all(torch.equal(out[k], w[k]) for k in w)
+
+
+@pytest.mark.parametrize("n, n_in, n_out", [(40, 70, 50), (20000, 64, 48), (3700, 3600, 48)])
+def test_a_row_that_is_not_finite_reaches_what_it_enters_and_no_more(n, n_in, n_out):
+    dy, xk, zk, w, x, z = backward_inputs("f16", n, n_in, n_out, 3, True, False)
+    want = U.call_linear_backward("f16", dy, xk, w, "silu", zk)
+    dy[n // 3, 5] = float("inf")
+    dx, dw, db = U.call_linear_backward("f16", dy, xk, w, "silu", zk)
+    keep = torch.arange(n, device="cuda") != n // 3
+    assert torch.equal(dx[keep], want[0][keep]) and not torch.isfinite(dx[n // 3]).any()
+    cols = torch.arange(n_out, device="cuda") != 5
+    assert torch.equal(dw[cols], want[1][cols]) and not torch.isfinite(dw[5]).any()
+    assert torch.equal(db[cols], want[2][cols]) and not torch.isfinite(db[5])
+
+
 def residual_block_without_checks(kind, s):
     """The block for a capture: guards are not looked at (that waits for the GPU), and every buffer stays held."""
     held, asked = [], U.guards_hold
