@@ -27,6 +27,8 @@
  *                             + update_density_grid_mean_and_bitfield :2362-2379
  *   ngp_render                Testbed::render_nerf / NerfTracer      src/testbed_nerf.cu:1827-1987, 1556-1761
  *   ngp_accumulate_tonemap    CudaRenderBuffer::accumulate + tonemap src/render_buffer.cu:635-691 (kernels :232,:533)
+ *   ngp_linear_*              layers of the widths tcnn's CutlassMLP serves (the network object of src/testbed.cu:3726-3727)
+ *   ngp_layer_norm_*, ngp_checkpoint_*  (no reference counterpart: layer norm, activations kept in 8 bits)
  *
  * Error behaviour mirrors the reference: where the reference throws
  * std::runtime_error (CUDA_CHECK_THROW, invalid arguments), these return a

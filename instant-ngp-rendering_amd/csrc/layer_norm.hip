@@ -34,66 +34,64 @@ __device__ __forceinline__ void group_sums(float (&v)[N], uint32_t G, float* par
 }
 
 constexpr uint32_t NORM_THREADS = 256;     // a workgroup's, unless a row's group is larger
-constexpr uint32_t NORM_GRID = 1u << 20;  // workgroups at most (a launch has fewer than 2^32 threads); they then go on
+constexpr uint32_t NORM_GRID = 1u << 20;  // workgroups at most side by side (a grid has fewer than 2^32 threads that way)
 
 // The mean, then the mean square of what is left of it (no cancellation), then the row.
 template <class T, int C>
 __global__ void __launch_bounds__(1024) k_norm_forward(ngp_layer_norm_args a, uint32_t G) {
 	__shared__ float part[2][16];
-	const uint32_t g = threadIdx.x % G, groups = blockDim.x / G;
-	for (size_t i0 = (size_t)blockIdx.x * groups; i0 < a.n; i0 += (size_t)gridDim.x * groups) {
-		const size_t i = i0 + threadIdx.x / G;
-		const bool here = i < a.n;
-		const T* x = static_cast<const T*>(a.x) + i * a.x_stride;
-		v8<T> raw[C];
-		uint32_t left[C];
-		float s[1] = {0.0f};
+	const uint32_t g = threadIdx.x % G;
+	const size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * (blockDim.x / G) + threadIdx.x / G;
+	const bool here = i < a.n;
+	const T* x = static_cast<const T*>(a.x) + i * a.x_stride;
+	v8<T> raw[C];
+	uint32_t left[C];
+	float s[1] = {0.0f};
 #pragma unroll
-		for (int c = 0; c < C; ++c) {
-			const uint32_t j = (c * G + g) * 8u;
-			left[c] = here && j < a.width ? a.width - j : 0u;
-			raw[c] = load8_raw(x + j, left[c]);
+	for (int c = 0; c < C; ++c) {
+		const uint32_t j = (c * G + g) * 8u;
+		left[c] = here && j < a.width ? a.width - j : 0u;
+		raw[c] = load8_raw(x + j, left[c]);
+	}
+#pragma unroll
+	for (int c = 0; c < C; ++c)
+#pragma unroll
+		for (int k = 0; k < 8; ++k) s[0] += widen(raw[c][k]);  // zeros past the row
+	group_sums(s, G, part[0]);
+	const float mean = s[0] / (float)a.width;
+	s[0] = 0.0f;
+#pragma unroll
+	for (int c = 0; c < C; ++c)
+#pragma unroll
+		for (int k = 0; k < 8; ++k) {
+			const float d = widen(raw[c][k]) - mean;
+			s[0] += (uint32_t)k < left[c] ? d * d : 0.0f;
 		}
+	group_sums(s, G, part[1]);
+	const float rstd = 1.0f / sqrtf(s[0] / (float)a.width + a.epsilon);
+	if (here && g == 0) {
+		if (a.mean) a.mean[i] = mean;
+		if (a.rstd) a.rstd[i] = rstd;
+	}
 #pragma unroll
-		for (int c = 0; c < C; ++c)
+	for (int c = 0; c < C; ++c) {
+		const uint32_t j = (c * G + g) * 8u;
+		float v[8], gamma[8], beta[8];
 #pragma unroll
-			for (int k = 0; k < 8; ++k) s[0] += widen(raw[c][k]);  // zeros past the row
-		group_sums(s, G, part[0]);
-		const float mean = s[0] / (float)a.width;
-		s[0] = 0.0f;
+		for (int k = 0; k < 8; ++k) gamma[k] = 1.0f, beta[k] = 0.0f;
+		if (left[c] && a.gamma) load8(a.gamma + j, left[c], gamma);
+		if (left[c] && a.beta) load8(a.beta + j, left[c], beta);
 #pragma unroll
-		for (int c = 0; c < C; ++c)
+		for (int k = 0; k < 8; ++k) v[k] = (widen(raw[c][k]) - mean) * rstd * gamma[k] + beta[k];
+		if (left[c]) store8(static_cast<T*>(a.y) + i * a.y_stride + j, left[c], v);
+		if (!a.y8.q) continue;
+		uint32_t top = 0;
 #pragma unroll
-			for (int k = 0; k < 8; ++k) {
-				const float d = widen(raw[c][k]) - mean;
-				s[0] += (uint32_t)k < left[c] ? d * d : 0.0f;
-			}
-		group_sums(s, G, part[1]);
-		const float rstd = 1.0f / sqrtf(s[0] / (float)a.width + a.epsilon);
-		if (here && g == 0) {
-			if (a.mean) a.mean[i] = mean;
-			if (a.rstd) a.rstd[i] = rstd;
-		}
-#pragma unroll
-		for (int c = 0; c < C; ++c) {
-			const uint32_t j = (c * G + g) * 8u;
-			float v[8], gamma[8], beta[8];
-#pragma unroll
-			for (int k = 0; k < 8; ++k) gamma[k] = 1.0f, beta[k] = 0.0f;
-			if (left[c] && a.gamma) load8(a.gamma + j, left[c], gamma);
-			if (left[c] && a.beta) load8(a.beta + j, left[c], beta);
-#pragma unroll
-			for (int k = 0; k < 8; ++k) v[k] = (widen(raw[c][k]) - mean) * rstd * gamma[k] + beta[k];
-			if (left[c]) store8(static_cast<T*>(a.y) + i * a.y_stride + j, left[c], v);
-			if (!a.y8.q) continue;
-			uint32_t top = 0;
-#pragma unroll
-			for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left[c] ? magnitude_bits(v[k]) : 0u);
-			const uint32_t scale = checkpoint_scale<T>(quad_max(top));
-			if (!left[c]) continue;
-			checkpoint_store8(a.y8.q + i * a.y8.q_stride + j, left[c], scale, v);
-			if (j % 32u == 0) a.y8.scale[i * a.y8.scale_stride + j / 32u] = (uint8_t)scale;
-		}
+		for (int k = 0; k < 8; ++k) top = max(top, (uint32_t)k < left[c] ? magnitude_bits(v[k]) : 0u);
+		const uint32_t scale = checkpoint_scale<T>(quad_max(top));
+		if (!left[c]) continue;
+		checkpoint_store8(a.y8.q + i * a.y8.q_stride + j, left[c], scale, v);
+		if (j % 32u == 0) a.y8.scale[i * a.y8.scale_stride + j / 32u] = (uint8_t)scale;
 	}
 }
 
@@ -268,8 +266,9 @@ static NormShape norm_shape(uint32_t n, uint32_t width, uint32_t most) {
 
 template <class T>
 static void norm_forward(const ngp_layer_norm_args& a, hipStream_t s) {
-	const NormShape p = norm_shape(a.n, a.width, 8);
-	const uint32_t rows = p.threads / p.G, grid = std::min((a.n + rows - 1) / rows, NORM_GRID);
+	const NormShape p = norm_shape(a.n, a.width, sizeof(T) == 4 ? 4 : 8);
+	const uint32_t rows = p.threads / p.G, sets = (a.n + rows - 1) / rows;
+	const dim3 grid(std::min(sets, NORM_GRID), (sets + NORM_GRID - 1) / NORM_GRID);
 	auto kernel = p.chunks == 1 ? k_norm_forward<T, 1> : p.chunks == 2 ? k_norm_forward<T, 2> : p.chunks == 4 ? k_norm_forward<T, 4> : k_norm_forward<T, 8>;
 	kernel<<<grid, p.threads, 0, s>>>(a, p.G);
 	NGP_HIP_CHECK(hipGetLastError());

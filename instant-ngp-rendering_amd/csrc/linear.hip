@@ -486,10 +486,10 @@ template <class T, int TILE, int BUFFERS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(ProductArgs dx, GradientOut<T> dx_out, uint32_t dx_blocks, ProductArgs dw,
                                                                           WeightsOut<T> dw_out, uint32_t dw_blocks, Sums sums) {
 	extern __shared__ __attribute__((aligned(16))) char lds[];
-	if (blockIdx.x < dx_blocks)
-		product_tile<T, GradientOut<T>, false, true, TILE, TILE, 64, BUFFERS>(dx, dx_out, blockIdx.x, dx_blocks, lds);
-	else if (blockIdx.x - dx_blocks < dw_blocks)
-		product_tile<T, WeightsOut<T>, true, true, TILE, TILE, 64, BUFFERS>(dw, dw_out, blockIdx.x - dx_blocks, dw_blocks, lds);
+	if (blockIdx.x < dw_blocks)  // first, as K is the rows: the longest to take
+		product_tile<T, WeightsOut<T>, true, true, TILE, TILE, 64, BUFFERS>(dw, dw_out, blockIdx.x, dw_blocks, lds);
+	else if (blockIdx.x - dw_blocks < dx_blocks)
+		product_tile<T, GradientOut<T>, false, true, TILE, TILE, 64, BUFFERS>(dx, dx_out, blockIdx.x - dw_blocks, dx_blocks, lds);
 	else
 		column_sums<PRODUCT_THREADS>(sums.part, sums.shares, sums.columns, sums.put, blockIdx.x - dx_blocks - dw_blocks);
 }
