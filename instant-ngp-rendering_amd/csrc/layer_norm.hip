@@ -97,11 +97,11 @@ __global__ void __launch_bounds__(1024) k_norm_forward(ngp_layer_norm_args a, ui
 
 // A workgroup takes every gridDim.x-th set of rows.  SUMS: it keeps its threads' columns of dgamma and dbeta in registers
 // meanwhile and leaves their sums over its rows in part_out[blockIdx.x][2][width].
-template <class T, int C, bool SUMS>
-__global__ void __launch_bounds__(NORM_THREADS) k_norm_backward(ngp_layer_norm_backward_args a, uint32_t G, float* __restrict__ part_out) {
+template <class T, int C, int THREADS, bool SUMS>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 3) k_norm_backward(ngp_layer_norm_backward_args a, uint32_t G, float* __restrict__ part_out) {
 	extern __shared__ float lds[];  // two shares of 32 floats, then the columns of the groups
 	const Kept<T> x{static_cast<const T*>(a.x), a.x_stride, a.x8.q, a.x8.scale, a.x8.q_stride, a.x8.scale_stride};
-	const uint32_t g = threadIdx.x % G, group = threadIdx.x / G, groups = NORM_THREADS / G;
+	const uint32_t g = threadIdx.x % G, group = threadIdx.x / G, groups = THREADS / G;
 	uint32_t left[C];
 	float gamma[C][8], dg[SUMS ? C : 1][8] = {}, db[SUMS ? C : 1][8] = {};
 #pragma unroll
@@ -167,12 +167,12 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_backward(ngp_layer_norm_b
 			if (groups > 1) {  // the groups' sums in their order
 				__syncthreads();
 #pragma unroll
-				for (int k = 0; k < 8; ++k) columns[k * NORM_THREADS + threadIdx.x] = v[k];
+				for (int k = 0; k < 8; ++k) columns[k * THREADS + threadIdx.x] = v[k];
 				__syncthreads();
 				if (group == 0)
 					for (uint32_t o = 1; o < groups; ++o)
 #pragma unroll
-						for (int k = 0; k < 8; ++k) v[k] += columns[k * NORM_THREADS + o * G + g];
+						for (int k = 0; k < 8; ++k) v[k] += columns[k * THREADS + o * G + g];
 			}
 			if (group == 0 && left[c]) store8(out + (size_t)h * a.width + (c * G + g) * 8u, left[c], v);
 		}
@@ -274,9 +274,10 @@ static void norm_forward(const ngp_layer_norm_args& a, hipStream_t s) {
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
-// Backward: half the chunks, since a thread keeps two sums per column.  Two workgroups of 256 per CU go through the rows
-// in turns.
-constexpr uint32_t NORM_IN_PASS = NORM_THREADS * 4 * 8;
+// Backward: a quarter of the chunks, since a thread keeps two sums per column.  As many workgroups per CU as their registers
+// allow, three of 256 or (rows over 4096) one of 512, go through the rows in turns (65536 rows of 2048 fp16: 201 us, with two
+// per CU 220, with four chunks per thread 266; 20000 rows of 6000 with four chunks of 256 threads 327 us).
+constexpr uint32_t NORM_IN_PASS = 512 * 2 * 8;
 struct NormBackwardPlan {
 	NormShape shape;
 	bool sums, in_pass;  // dgamma or dbeta wanted; by k_norm_backward
@@ -284,9 +285,11 @@ struct NormBackwardPlan {
 };
 static NormBackwardPlan backward_plan(const ngp_layer_norm_backward_args& a) {
 	NormBackwardPlan p{norm_shape(a.n, a.width, 2), a.dgamma || a.dbeta, a.width <= NORM_IN_PASS, 0, 0};
-	while (p.in_pass && p.shape.G > NORM_THREADS) p.shape.G /= 2, p.shape.chunks *= 2;
-	const uint32_t rows = NORM_THREADS / std::min(p.shape.G, NORM_THREADS);
-	p.grid = std::max(1u, std::min((a.n + rows - 1) / rows, 512u));
+	while (p.in_pass && p.shape.G > (a.width <= 4096 ? 256u : 512u)) p.shape.G /= 2, p.shape.chunks *= 2;
+	p.shape.threads = std::max(p.shape.G, NORM_THREADS);
+	const uint32_t rows = std::max(1u, p.shape.threads / p.shape.G), most = p.shape.threads > 256 ? 256 : 768;
+	const uint32_t sets = std::max(1u, (a.n + rows - 1) / rows), turns = (sets + most - 1) / most;
+	p.grid = (sets + turns - 1) / turns;
 	p.parts = p.in_pass ? p.grid : std::max(1u, std::min(256u, a.n / 16u));
 	return p;
 }
@@ -298,8 +301,10 @@ size_t layer_norm_backward_workspace(const ngp_layer_norm_backward_args& a) {
 
 template <class T, int C>
 static void launch_backward(const ngp_layer_norm_backward_args& a, const NormBackwardPlan& p, float* part, hipStream_t s) {
-	auto kernel = part ? k_norm_backward<T, C, true> : k_norm_backward<T, C, false>;
-	kernel<<<p.grid, NORM_THREADS, (64 + (p.shape.G < NORM_THREADS ? 8 * NORM_THREADS : 0)) * sizeof(float), s>>>(a, p.shape.G, part);
+	const uint32_t threads = p.shape.threads;
+	auto kernel = threads > 256 ? (part ? k_norm_backward<T, C, 512, true> : k_norm_backward<T, C, 512, false>)
+	                            : (part ? k_norm_backward<T, C, 256, true> : k_norm_backward<T, C, 256, false>);
+	kernel<<<p.grid, threads, (64 + (p.shape.G < threads ? 8 * threads : 0)) * sizeof(float), s>>>(a, p.shape.G, part);
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
@@ -309,8 +314,7 @@ static void norm_backward(const ngp_layer_norm_backward_args& a, hipStream_t s) 
 	float* part = p.sums ? static_cast<float*>(a.workspace) : nullptr;
 	if (p.in_pass && (part || (a.dx && a.n))) {
 		if (p.shape.chunks == 1) launch_backward<T, 1>(a, p, part, s);
-		else if (p.shape.chunks == 2) launch_backward<T, 2>(a, p, part, s);
-		else launch_backward<T, 4>(a, p, part, s);
+		else launch_backward<T, 2>(a, p, part, s);
 	}
 	if (!p.in_pass && part) {
 		const size_t each = ((size_t)a.n + p.parts - 1) / p.parts;

@@ -738,17 +738,23 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : NI + NO > 128 ? 2 : 3
 	// the weights as dx's Q: row = input, k = output
 	const uint32_t strip = wave % STRIPS, nt0 = wave / STRIPS * NT;
 	s16x8 w[NT][NO / 16] = {};
-	if (a.dx)
+	if (a.dx) {
+#ifdef __HIP_DEVICE_COMPILE__
+		// through a buffer, which gives zeros for what is not there: with a condition on the value the compiler puts a branch
+		// and a wait around each of these loads (20 us in all)
+		const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(a.w), (short)0, 0x7fffffff, 0x00027000);
 #pragma unroll
 		for (int t = 0; t < NT; ++t)
 #pragma unroll
 			for (int s = 0; s < NO / 16; ++s)
 #pragma unroll
-				for (int k = 0; k < 8; ++k) {  // (no branch among the loads: what is not there is read as another and dropped)
+				for (int k = 0; k < 8; ++k) {
 					const uint32_t row = (nt0 + t) * 32u + (lane & 31u), out = s * 16u + 8u * (lane >> 5) + k;
-					const T v = a.w[min(out, a.n_out - 1u) * a.w_stride + min(row, a.n_in - 1u)];
-					w[t][s][k] = row < a.n_in && out < a.n_out ? __builtin_bit_cast(short, v) : (short)0;
+					const uint32_t at = row < a.n_in && out < a.n_out ? (out * (uint32_t)a.w_stride + row) * 2u : 0xfffffff0u;
+					w[t][s][k] = (short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, at, 0, 0);
 				}
+#endif
+	}
 
 	f32x16 dw[WT] = {};
 	float db[8] = {};
@@ -838,14 +844,15 @@ __global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : NI + NO > 128 ? 2 : 3
 					float v[8];
 					eight(c[t], h, v);
 					if (i >= a.n || j >= a.n_in) continue;
+					const uint32_t left = EVEN ? 8u : a.n_in - j;
 					if (a.x_act != NGP_ACT_NONE) {
 						float s[8];
-						a.x.at8(i, j, a.n_in - j, s);
+						a.x.at8(i, j, left, s);
 						act_slopes(a.x_act, s);
 #pragma unroll
 						for (int k = 0; k < 8; ++k) v[k] *= s[k];
 					}
-					store8(a.dx + i * a.dx_stride + j, a.n_in - j, v);
+					store8(a.dx + i * a.dx_stride + j, left, v);
 				}
 		}
 		if (a.want_dw)
