@@ -497,7 +497,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(Produc
 // 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
 // reads its next fragments and asks for a stage of K ahead, and then they change places.  A barrier after each half keeps
 // the two sets of four waves in opposite phases.  K goes through 128 KiB of LDS in stages of DEEP, each multiplied in steps
-// of 32: two buffers of 64 or four of 32.
+// of 32: two buffers of 64 or four of 32.  Measured over 16384 rows of 2048 x 8192 (0.55 TFLOP, bf16): dW
+// 455 us (1.2 PFLOP/s, the matrix cores busy for 72 % of the cycles at the clock that they then run at), y and dx 595 us, of
+// which about 0.14 ms are the epilogues: bound by their instructions (28 per value with a gelu and a checkpoint), with the CU to
+// themselves.
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int DEEP>
 __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a, Out out) {
 	constexpr int BM = 256, BN = 256, TM = 4, TN = 2, BUFFERS = 128 / DEEP;
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_rows(const T* __restrict__ 
 // workgroups of four waves take ROWS rows at a time: dz and the layer's input go to LDS in 16 bits ([row][feature], from
 // where dx reads dz along its rows and dW reads both transposed), the weights' fragments and the workgroup's share of dW stay
 // in registers, the next rows are on their way from memory meanwhile.  dW and db leave as a share per workgroup.
-// 64 -> 64 over 2^18 rows moves 134 MB instead of the 233 MB of separate passes.
+// 64 -> 64 over 2^18 rows moves 134 MB instead of the 233 MB of separate passes: 33 us (4.1 TB/s), and 5 to join the shares.
 template <class T>
 struct NarrowArgs {
 	Kept<T> dy, z, x;
@@ -1053,12 +1056,12 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K, int only = 0) {
 	return best;
 }
 
-template <class Out>
-static void launch_product(void (*kernel)(ProductArgs, Out), uint32_t threads, uint32_t lds, const ProductArgs& a, const Out& out,
-                           hipStream_t s) {
-	if (lds > 65536)
-		NGP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-	kernel<<<a.tiles_m * a.tiles_n * a.splits, threads, lds, s>>>(a, out);
+// A kernel's LDS past the default of 64 KiB (its own static LDS counted) has to be allowed once per device.
+template <class... Args>
+static void launch_lds(void (*kernel)(Args...), uint32_t blocks, uint32_t threads, uint32_t lds, hipStream_t s, Args... args) {
+	if (lds >= 65536)
+		NGP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+	kernel<<<blocks, threads, lds, s>>>(args...);
 	NGP_HIP_CHECK(hipGetLastError());
 }
 
@@ -1083,10 +1086,13 @@ static bool is_short(const ProductPlan& plan) { return plan.k_each <= 2 * PRODUC
 
 template <class T, class Out, bool P_BY_K, bool Q_BY_K>
 static void product(const ProductPlan& plan, const ProductArgs& a, const Out& out, hipStream_t s) {
-	if (plan.tile == 256) launch_product(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, WIDE_THREADS, 131072, a, out, s);
-	else if (plan.tile == 128) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 128, 2>, PRODUCT_THREADS, 2 * 32768, a, out, s);
-	else if (is_short(plan)) launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 2>, PRODUCT_THREADS, 2 * 16384, a, out, s);
-	else launch_product(k_product<T, Out, P_BY_K, Q_BY_K, 64, 3>, PRODUCT_THREADS, 3 * 16384, a, out, s);
+	const uint32_t blocks = a.tiles_m * a.tiles_n * a.splits;
+	// (rows along k come 128 bytes at a time from stages of 64: half the requests to L2, y of 16384 x 2048 x 8192 666 us, 704 with
+	// stages of 32; with an operand by k, whose lines are long either way, stages of 32 ask further ahead: dx 655 us, 673)
+	if (plan.tile == 256) launch_lds(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, blocks, WIDE_THREADS, 131072, s, a, out);
+	else if (plan.tile == 128) launch_lds(k_product<T, Out, P_BY_K, Q_BY_K, 128, 2>, blocks, PRODUCT_THREADS, 2 * 32768, s, a, out);
+	else if (is_short(plan)) launch_lds(k_product<T, Out, P_BY_K, Q_BY_K, 64, 2>, blocks, PRODUCT_THREADS, 2 * 16384, s, a, out);
+	else launch_lds(k_product<T, Out, P_BY_K, Q_BY_K, 64, 3>, blocks, PRODUCT_THREADS, 3 * 16384, s, a, out);
 	if (a.splits > 1) join<T>(a.partial, a.splits, a.M, a.N, out, s);
 }
 
@@ -1229,12 +1235,11 @@ static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipSt
 		const uint32_t dx_blocks = dx_args.tiles_m * dx_args.tiles_n * dx_args.splits, dw_blocks = dw_args.tiles_m * dw_args.tiles_n * dw_args.splits;
 		const uint32_t blocks = dx_blocks + dw_blocks + (sums.columns + 15) / 16;
 		if (dx_plan.tile == 128)
-			k_backward_products<T, 128, 2><<<blocks, PRODUCT_THREADS, 2 * 32768, s>>>(dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
+			launch_lds(k_backward_products<T, 128, 2>, blocks, PRODUCT_THREADS, 2 * 32768, s, dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
 		else if (is_short(dx_plan) && is_short(dw_plan))
-			k_backward_products<T, 64, 2><<<blocks, PRODUCT_THREADS, 2 * 16384, s>>>(dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
+			launch_lds(k_backward_products<T, 64, 2>, blocks, PRODUCT_THREADS, 2 * 16384, s, dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
 		else
-			k_backward_products<T, 64, 3><<<blocks, PRODUCT_THREADS, 3 * 16384, s>>>(dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
-		NGP_HIP_CHECK(hipGetLastError());
+			launch_lds(k_backward_products<T, 64, 3>, blocks, PRODUCT_THREADS, 3 * 16384, s, dx_args, dx_out, dx_blocks, dw_args, dw_out, dw_blocks, sums);
 		if (dx_args.splits > 1) join<T>(dx_args.partial, dx_args.splits, a.n, a.n_in, dx_out, s);
 		if (dw_args.splits > 1) join<T>(dw_args.partial, dw_args.splits, a.n_out, a.n_in, dw_out, s);
 		return room.bytes;

@@ -55,7 +55,8 @@ def check_checkpoint(c8, want, tol, kind):
 # n, n_in, n_out: a row, tiles' edges on both sides, odd widths, few and many rows
 SHAPES = [(1, 1, 1), (1, 64, 64), (1, 1024, 520), (2, 33, 65), (5, 7, 3), (16, 256, 48), (17, 40, 130), (33, 8, 31), (63, 65, 127),
           (64, 64, 64), (65, 72, 136), (129, 257, 255), (200, 512, 264), (257, 96, 1), (300, 1, 300), (1000, 333, 77),
-          (127, 2048, 64), (513, 128, 640), (2049, 64, 16), (1, 4096, 4500), (3, 2500, 40), (16, 16384, 96), (13, 2111, 36)]
+          (127, 2048, 64), (513, 128, 640), (2049, 64, 16), (1, 4096, 4500), (3, 2500, 40), (16, 16384, 96), (13, 2111, 36),
+          (3, 65536, 40), (40, 24, 65536)]
 
 
 def forward_reference(x, w, b, name, r):
