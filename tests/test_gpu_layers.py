@@ -274,6 +274,22 @@ def test_backward_of_some_gradients_only():
         assert torch.equal(some[k], every[k]) and all(v is None for i, v in enumerate(some) if i != k)
 
 
+# what a call does not need may be absent, what it has no use for may be there
+@pytest.mark.parametrize("n, n_in, n_out", [(150, 88, 40), (16400, 64, 40), (16401, 45, 91), (4100, 3600, 264)])
+def test_backward_with_as_little_and_as_much_as_is_allowed(n, n_in, n_out):
+    dy, xk, zk, w, x, z = backward_inputs("f16", n, n_in, n_out, 4, False, False)
+    every = U.call_linear_backward("f16", dy, xk, w, "none", None)
+    check_backward("f16", every, dy, x, z, w, "none", "none")
+    for got in (U.call_linear_backward("f16", dy, xk, w, "none", zk), U.call_linear_backward("f16", dy, xk, w, "none", U.call_store("f16", zk))):
+        assert all(torch.equal(g, e) for g, e in zip(got, every))
+    got = U.call_linear_backward("f16", dy, None, w, "none", None, dw=None)
+    assert got[1] is None
+    check_backward("f16", got, dy, x, z, w, "none", "none")  # (one product alone may take other tiles than two together)
+    got = U.call_linear_backward("f16", dy, xk, None, "none", None, dx=None, db=None, n_in=n_in)
+    assert got[0] is None and got[2] is None
+    check_backward("f16", got, dy, x, z, w, "none", "none")
+
+
 def test_no_rows():
     for kind in ("f16", "bf16"):
         t = U.TYPES[kind][1]
