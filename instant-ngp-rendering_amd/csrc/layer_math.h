@@ -28,8 +28,8 @@ __device__ __forceinline__ float act_rcp(float x) { return __builtin_amdgcn_rcpf
 // cost of a rational form of the tail: a 256 x 256 tile's 65536 gelus are a quarter of its time at K = 2048):
 //  * the tail Phi(-a) = 2^L(a) for 0 <= a <= 8, degree 8: relative error 5.3e-6, 1.1e-5 with fp32 rounding.  Past 8 nothing
 //    is left of it (6e-16).
-//  * the gelu's slope at -a, Phi(-a) - a phi(a) = exp(-a^2 / 2) S(a), degree 9: off by 2.6e-7 (it enters sums over all rows,
-//    which are held in fp32), and by less than 6e-8 past a = 6, where S(6) stands for S(a).
+//  * the gelu's slope at -a, Phi(-a) - a phi(a) = exp(-a^2 / 2) S(a), degree 9: off by 2.6e-7, 3.7e-7 with fp32 rounding (it
+//    enters sums over all rows, which are held in fp32), and by less than 6e-8 past a = 6, where S(6) stands for S(a).
 __device__ __forceinline__ float gelu_value(float z) {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
 	const float a = fminf(fabsf(z), 8.0f);
 	float l = 7.427881287228275e-08f;
@@ -41,7 +41,8 @@ __device__ __forceinline__ float gelu_value(float z) {  // z Phi(z) = max(z, 0) 
 	l = __builtin_fmaf(l, a, -0.45819584686337644f);
 	l = __builtin_fmaf(l, a, -1.1513217395138415f);
 	l = __builtin_fmaf(l, a, -0.9999923663359365f);
-	return __builtin_fmaf(-a, __builtin_amdgcn_exp2f(l), 0.5f * (z + fabsf(z)));  // max(z, 0) that keeps a NaN
+	// max(z, 0) that keeps a NaN, in halves: z + |z| overflows from 2^127 on
+	return __builtin_fmaf(-a, __builtin_amdgcn_exp2f(l), __builtin_fmaf(0.5f, fabsf(z), 0.5f * z));
 }
 __device__ __forceinline__ float gelu_slope(float z) {
 	const float a = fminf(fabsf(z), 6.0f), bell = __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);  // -log2(e) / 2
