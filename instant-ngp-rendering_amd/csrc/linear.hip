@@ -228,13 +228,14 @@ struct Stage {
 		const i32x4 rsrc = {(int)(uint32_t)from, (int)(uint32_t)(from >> 32), (int)end, 0x00027000};
 		const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_ptr)lds) + (threadIdx.x & ~63u) * 16u);
 		// not the builtin: the compiler then waits for every load into LDS before each transposed read from it, whichever
-		// buffer they are for.  The waits are written out where the stages change; nothing is loaded into registers here, and
-		// m0 (the LDS address, a register the compiler only ever sets right before it needs it) is set in the same block.
+		// buffer they are for.  The waits are written out where the stages change; nothing is loaded into registers here.  The
+		// block says what it writes, m0 (the LDS address) and memory, so that no access to LDS or memory moves over it.
 #pragma unroll
 		for (int l = 0; l < LOADS; ++l)
 			asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
 			             :
-			             : "s"(to + l * THREADS * 16), "v"(at[l]), "s"(rsrc));
+			             : "s"(to + l * THREADS * 16), "v"(at[l]), "s"(rsrc)
+			             : "m0", "memory");
 	}
 };
 
