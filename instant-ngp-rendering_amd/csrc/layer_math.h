@@ -152,10 +152,6 @@ __device__ __forceinline__ uint32_t checkpoint_scale(uint32_t max_bits) {
 }
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 // ldexp keeps the power of two exact over the whole range (133 - scale reaches past the largest float's exponent)
-__device__ __forceinline__ int checkpoint_q(float v, uint32_t scale) {
-	const float q = rintf(ldexpf(v, 133 - (int)scale));
-	return scale == 255u ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
 __device__ __forceinline__ float checkpoint_value(int q, uint32_t scale) {
 	return scale == 255u ? __uint_as_float(0x7fc00000u) : ldexpf((float)q, (int)scale - 133);
 }

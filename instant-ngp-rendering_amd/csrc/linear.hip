@@ -292,7 +292,7 @@ __device__ __forceinline__ void finish_block(const Out& out, size_t i, uint32_t 
 
 // Where a workgroup works.  Workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring tiles, eight tile
 // rows deep, so that its L2 holds what they share.
-template <int BM, int BN>
+template <int TILE>
 struct Place {
 	uint32_t split, n0;
 	size_t m0, k0, k1;
@@ -302,8 +302,8 @@ struct Place {
 		split = id / tiles;
 		const uint32_t tile = id % tiles, group = tile / (8u * a.tiles_n), first = group * 8u, deep = min(8u, a.tiles_m - first);
 		const uint32_t in_group = tile - group * 8u * a.tiles_n;
-		m0 = (size_t)(first + in_group % deep) * BM;
-		n0 = in_group / deep * BN;
+		m0 = (size_t)(first + in_group % deep) * TILE;
+		n0 = in_group / deep * TILE;
 		// rows along k are filled up to 8 with zeros; lines past K are not there, which the loads know
 		k0 = split * a.k_each;
 		k1 = min(k0 + a.k_each, (a.K + 7u) & ~(size_t)7u);
@@ -401,20 +401,20 @@ __device__ __forceinline__ void meet() {
 	asm volatile("" ::: "memory");
 }
 
-// BM x BN of C per workgroup of four waves, two by two; K in stages of 64 through BUFFERS LDS buffers: while the matrix cores
+// TILE x TILE of C per workgroup of four waves, two by two; K in stages of 64 through BUFFERS LDS buffers: while the matrix cores
 // work on one stage, the others are on their way from memory into LDS without passing registers.  P's rows are the matrix
 // instruction's columns and Q's its rows, so that a lane ends up with neighbouring columns of C.
-template <class T, class Out, bool P_BY_K, bool Q_BY_K, int BM, int BN, int DEEP, int BUFFERS>
+template <class T, class Out, bool P_BY_K, bool Q_BY_K, int TILE, int BUFFERS>
 __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& out, uint32_t block, uint32_t blocks, char* lds) {
-	constexpr int TM = BM / 64, TN = BN / 64;  // 32 x 32 tiles per wave
-	typedef Stage<T, BM, P_BY_K, DEEP, PRODUCT_THREADS> PStage;
-	typedef Stage<T, BN, Q_BY_K, DEEP, PRODUCT_THREADS> QStage;
+	constexpr int DEEP = PRODUCT_K, TM = TILE / 64, TN = TILE / 64;  // 32 x 32 tiles per wave
+	typedef Stage<T, TILE, P_BY_K, DEEP, PRODUCT_THREADS> PStage;
+	typedef Stage<T, TILE, Q_BY_K, DEEP, PRODUCT_THREADS> QStage;
 	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
 	static_assert(4 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
 
-	const Place<BM, BN> at(a, block, blocks);
+	const Place<TILE> at(a, block, blocks);
 	const uint32_t wave = threadIdx.x / 64u;
-	const uint32_t wm = wave / 2u * (BM / 2), wn = wave % 2u * (BN / 2);
+	const uint32_t wm = wave / 2u * (TILE / 2), wn = wave % 2u * (TILE / 2);
 	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + DEEP - 1) / DEEP);
 
 	WriteOut<T, Out, TM, TN> write_out(a, out, at.m0 + wm, at.n0 + wn);
@@ -422,8 +422,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& ou
 	if (stages) {
 		PStage ps;
 		QStage qs;
-		Fragments<PStage, BM, P_BY_K, DEEP, TM> pf;
-		Fragments<QStage, BN, Q_BY_K, DEEP, TN> qf;
+		Fragments<PStage, TILE, P_BY_K, DEEP, TM> pf;
+		Fragments<QStage, TILE, Q_BY_K, DEEP, TN> qf;
 		ps.begin(a.p, at.m0, a.M, at.k0, a.K);
 		qs.begin(a.q, at.n0, a.N, at.k0, a.K);
 		pf.begin(wm);
@@ -473,7 +473,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, const Out& ou
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int TILE, int BUFFERS>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_product(ProductArgs a, Out out) {
 	extern __shared__ __attribute__((aligned(16))) char lds[];
-	product_tile<T, Out, P_BY_K, Q_BY_K, TILE, TILE, 64, BUFFERS>(a, out, blockIdx.x, gridDim.x, lds);
+	product_tile<T, Out, P_BY_K, Q_BY_K, TILE, BUFFERS>(a, out, blockIdx.x, gridDim.x, lds);
 }
 
 // A layer's dx and dW, and the join of db's shares, side by side in one launch: none of them fills the GPU in layers whose
@@ -488,9 +488,9 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(Produc
                                                                           WeightsOut<T> dw_out, uint32_t dw_blocks, Sums sums) {
 	extern __shared__ __attribute__((aligned(16))) char lds[];
 	if (blockIdx.x < dw_blocks)  // first, as K is the rows: the longest to take
-		product_tile<T, WeightsOut<T>, true, true, TILE, TILE, 64, BUFFERS>(dw, dw_out, blockIdx.x, dw_blocks, lds);
+		product_tile<T, WeightsOut<T>, true, true, TILE, BUFFERS>(dw, dw_out, blockIdx.x, dw_blocks, lds);
 	else if (blockIdx.x - dw_blocks < dx_blocks)
-		product_tile<T, GradientOut<T>, false, true, TILE, TILE, 64, BUFFERS>(dx, dx_out, blockIdx.x - dw_blocks, dx_blocks, lds);
+		product_tile<T, GradientOut<T>, false, true, TILE, BUFFERS>(dx, dx_out, blockIdx.x - dw_blocks, dx_blocks, lds);
 	else
 		column_sums<PRODUCT_THREADS>(sums.part, sums.shares, sums.columns, sums.put, blockIdx.x - dx_blocks - dw_blocks);
 }
@@ -504,14 +504,14 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(Produc
 // 95 us of them, and 3 bytes written, 80 us (a 28th fewer instructions changed nothing for y and 1 % for dx).
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int DEEP>
 __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a, Out out) {
-	constexpr int BM = 256, BN = 256, TM = 4, TN = 2, BUFFERS = 128 / DEEP;
-	typedef Stage<T, BM, P_BY_K, DEEP, WIDE_THREADS> PStage;
-	typedef Stage<T, BN, Q_BY_K, DEEP, WIDE_THREADS> QStage;
+	constexpr int TILE = 256, TM = 4, TN = 2, BUFFERS = 128 / DEEP;
+	typedef Stage<T, TILE, P_BY_K, DEEP, WIDE_THREADS> PStage;
+	typedef Stage<T, TILE, Q_BY_K, DEEP, WIDE_THREADS> QStage;
 	constexpr int STAGE = PStage::BYTES + QStage::BYTES, LOADS = PStage::LOADS + QStage::LOADS;
 	static_assert(8 * STRIP<TN> * 4 <= BUFFERS * STAGE, "the stages' LDS holds the strips");
 	extern __shared__ __attribute__((aligned(16))) char lds[];
 
-	const Place<BM, BN> at(a, blockIdx.x, gridDim.x);
+	const Place<TILE> at(a, blockIdx.x, gridDim.x);
 	const uint32_t wave = threadIdx.x / 64u;
 	const uint32_t wm = wave / 4u * 128u, wn = wave % 4u * 64u;
 	const uint32_t stages = (uint32_t)((at.k1 - at.k0 + DEEP - 1) / DEEP);
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a,
 	if (stages) {
 		PStage ps;
 		QStage qs;
-		Fragments<PStage, BM, P_BY_K, DEEP, TM> pf;
-		Fragments<QStage, BN, Q_BY_K, DEEP, TN> qf;
+		Fragments<PStage, TILE, P_BY_K, DEEP, TM> pf;
+		Fragments<QStage, TILE, Q_BY_K, DEEP, TN> qf;
 		ps.begin(a.p, at.m0, a.M, at.k0, a.K);
 		qs.begin(a.q, at.n0, a.N, at.k0, a.K);
 		pf.begin(wm);
@@ -1001,10 +1001,9 @@ __global__ void __launch_bounds__(256) k_prepare(MakeDz<T> dz, LayOut<T> a, LayO
 static size_t up16(size_t b) { return (b + 15) & ~(size_t)15; }
 static uint32_t up8(uint32_t w) { return (w + 7u) & ~7u; }
 
-// The workspace as a call deals it out; without `run` nothing is launched and only the size is counted.
+// The workspace as a call deals it out, and how much of it is taken (the size to ask for, where nothing is launched).
 struct Room {
 	char* at;
-	bool run;
 	size_t bytes = 0;
 	template <class U>
 	U* take(size_t count) {
@@ -1057,7 +1056,8 @@ static ProductPlan plan_product(size_t M, uint32_t N, size_t K, int only = 0) {
 	return best;
 }
 
-// A kernel's LDS past the default of 64 KiB (its own static LDS counted) has to be allowed once per device.
+// A kernel's LDS past the default of 64 KiB (its own static LDS counted) has to be allowed, on each device that it runs on: at
+// every launch, so that nothing is kept between calls.
 template <class... Args>
 static void launch_lds(void (*kernel)(Args...), uint32_t blocks, uint32_t threads, uint32_t lds, hipStream_t s, Args... args) {
 	if (lds >= 65536)
@@ -1124,7 +1124,7 @@ constexpr uint32_t NARROW_WIDTH = 128, NARROW_ROWS = 16384;
 
 template <class T>
 static size_t linear_forward(const ngp_linear_args& a, bool run, hipStream_t s) {
-	Room room{static_cast<char*>(a.workspace), run};
+	Room room{static_cast<char*>(a.workspace)};
 	if (!a.n) return 0;
 	const ForwardOut<T> out{a.bias, static_cast<const T*>(a.residual), static_cast<T*>(a.y), static_cast<T*>(a.z), a.z8,
 	                        a.residual_stride, a.y_stride, a.z_stride, a.activation};
@@ -1164,7 +1164,7 @@ static void launch_narrow(const NarrowArgs<T>& a, uint32_t grid, hipStream_t s) 
 }
 template <class T>
 static size_t narrow_backward(const ngp_linear_backward_args& a, bool run, hipStream_t s) {
-	Room room{static_cast<char*>(a.workspace), run};
+	Room room{static_cast<char*>(a.workspace)};
 	const bool ni = a.n_in > 64, no = a.n_out > 64;
 	const uint32_t grid = ni && no ? 256 : 512;
 	const size_t columns = (size_t)a.n_out * (up8(a.n_in) + 1);
@@ -1186,7 +1186,7 @@ static size_t narrow_backward(const ngp_linear_backward_args& a, bool run, hipSt
 template <class T>
 static size_t linear_backward(const ngp_linear_backward_args& a, bool run, hipStream_t s) {
 	if (a.n >= NARROW_ROWS && a.n_in <= NARROW_WIDTH && a.n_out <= NARROW_WIDTH && (a.dx || a.dweights)) return narrow_backward<T>(a, run, s);
-	Room room{static_cast<char*>(a.workspace), run};
+	Room room{static_cast<char*>(a.workspace)};
 	const bool want_dx = a.dx && a.n, want_dw = a.dweights;
 	const Kept<T> x = kept<T>(a.x, a.x_stride, a.x8);
 	// dz where it has to be made, or copied into rows that the products can read
