@@ -562,7 +562,10 @@ ngp_status ngp_accumulate_tonemap(const float* frame, float* accum, float* out, 
  *  - Workspaces: the matching *_workspace call says how many bytes the same arguments need (0: none); 16-byte aligned,
  *    owned by one call at a time (two streams or captured graphs that may run together need one each).
  *  - Sums, means and statistics are held in fp32; sums over rows are taken in a fixed order (the same result every time).
- *  - Non-finite values follow the formulas. */
+ *    What leaves fp32's range on the way is infinite (a norm's row whose deviations are over 1.8e19 has rstd 0).
+ *  - Non-finite values follow the formulas (-inf times 0 is a NaN in gelu and silu; the relu's slope at a NaN is 0).
+ *  - Activations and slopes are off by less than the 16-bit types' half step: exponentials by 2^-23 (1 + |z|) relative, the gelu's
+ *    tail by 1.2e-5 relative (5e-15 past z = -8), its slope by 4e-7; results below 2^-126 may be 0. */
 enum { NGP_TYPE_F32 = 0, NGP_TYPE_F16 = 1, NGP_TYPE_BF16 = 2 };
 enum {
 	NGP_ACT_NONE = 0, /* 0..3 as ENerfActivation (common.h:90-95) */
@@ -577,9 +580,11 @@ enum {
 /* Activations kept in 8 bits: 32 consecutive features of a row (the last block of a row may be shorter) share a power of
  * two.  scale = the fp32 exponent field of the block's largest magnitude (at least 109 in NGP_TYPE_F16, whose step 2^-24 is
  * the type's smallest number); q = rint(v * 2^(133 - scale)), at most 127 in magnitude; a value stands for
- * q * 2^(scale - 133), which NGP_TYPE_F16 and NGP_TYPE_BF16 hold exactly: off by at most 2^(scale - 134), half a step,
- * except within half a step of the block's upper end, where it is off by less than one.  A block with a non-finite value
- * has scale 255 and stands for NaN throughout.  q: [n][q_stride], scale: [n][scale_stride] (one byte per 32 features);
+ * q * 2^(scale - 133): off by at most 2^(scale - 134), half a step, except within half a step of the block's upper end, where
+ * it is off by less than one.  NGP_TYPE_BF16 holds it exactly, and so does NGP_TYPE_F16 up to scale 142; a larger one, of z8 or
+ * y8 kept from fp32 values over 65504, is infinite where it is rounded to NGP_TYPE_F16 (ngp_checkpoint_load, an operand of a
+ * product) and as it is where a slope or a norm's gradient is taken from it.  A block with a non-finite value has scale 255 and
+ * stands for NaN throughout.  q: [n][q_stride], scale: [n][scale_stride] (one byte per 32 features);
  * bytes past a row's width (and past its last block's scale) are neither read nor written. */
 typedef struct ngp_checkpoint8 {
 	int8_t* q;
@@ -611,8 +616,9 @@ ngp_status ngp_linear_forward(const ngp_linear_args* args, ngp_stream stream);
 /* With p = x if x_activation is NGP_ACT_NONE, else x holds the pre-activation p of the layer below and this layer's input
  * was act_x(p), rounded to `type`:
  *   dz = dy act'(z), dx = (dz weights) act_x'(p), dweights = dz^T act_x(p), dbias = the sum of dz over the rows.
- * dz is rounded to `type` where it enters a product (the matrix cores' operands; dbias sums it in fp32).  The residual's
- * gradient is dy itself.  dx, dweights and dbias may each be null. */
+ * dz is rounded to `type` where it enters a product, for dweights in NGP_TYPE_F32 too (the matrix cores' operands; dbias sums it
+ * in fp32): half a step of each term, and in NGP_TYPE_F16 a dz over 65504 is infinite and one below 2^-25 is 0, so gradients
+ * that come near either are scaled by the caller (dx, dweights and dbias are linear in dy).  The residual's gradient is dy itself.  dx, dweights and dbias may each be null. */
 typedef struct ngp_linear_backward_args {
 	uint32_t n;
 	uint32_t n_in, n_out;

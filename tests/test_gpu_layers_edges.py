@@ -116,3 +116,32 @@ def test_activations_of_every_value(name, kind):
                                            x_activation=name, db=None)
         between(dx[plain], slope(name, z)[plain], slope_error(name, z)[plain], t, (name, "dx"))
         between(dw[plain], value(name, z)[plain], value_error(name, z)[plain], t, (name, "dw"))
+
+
+@pytest.mark.parametrize("n", [3, 40, 300])
+def test_checkpoints_of_sums_beyond_the_type(n):
+    """z8 and y8 are kept from fp32: past float16's range they are infinite as float16, and what they are for a slope."""
+    x, w = torch.full((n, 64), 1000.0, dtype=torch.float16, device="cuda"), torch.full((40, 64), 16.0, dtype=torch.float16, device="cuda")
+    w[1::2] *= -1
+    z8 = U.new8(n, 40)
+    y = U.call_linear("f16", x, w, None, "none", z8=z8)
+    z = 1000.0 * 16 * 64 * torch.tensor([1.0, -1.0], device="cuda").repeat(n, 20)
+    assert torch.equal(y.float(), z * math.inf)
+    q, e = U.store(z.double(), "f16")
+    assert torch.equal(z8[0], q) and torch.equal(z8[1], e) and (e == 127 + 19).all()  # 2^19 < 1024000 < 2^20
+    assert torch.equal(U.call_load("f32", z8, 40).double(), U.load(q, e))
+    assert torch.equal(U.call_load("f16", z8, 40).float(), z * math.inf)
+    dy = torch.ones(n, 40, dtype=torch.float16, device="cuda")
+    for name in ("relu", "gelu", "silu", "logistic"):
+        _, dw, db = U.call_linear_backward("f16", dy, torch.ones_like(x), w, name, z8, dx=None, dw_kind="f32")
+        slope_ = torch.zeros(40, device="cuda") if name == "logistic" else (z[0] > 0).float()
+        assert torch.equal(db, n * slope_) and torch.equal(dw, (n * slope_)[:, None].expand(40, 64))
+    # a norm's y8, with a gain that leaves the type
+    v = torch.tensor([1.0, -1.0], dtype=torch.float16, device="cuda").repeat(n, 32)
+    y8 = U.new8(n, 64)
+    y, mean, rstd = U.call_layer_norm("f16", v, torch.full((64,), 1e6, device="cuda"), eps=0.0, y8=y8)
+    assert torch.equal(y.float(), v.float() * math.inf) and (mean == 0).all() and (rstd == 1).all()
+    q, e = U.store(v.double() * 1e6, "f16")
+    assert torch.equal(y8[0], q) and torch.equal(y8[1], e)
+    dx, dgamma, dbeta = U.call_layer_norm_backward("f16", torch.ones_like(v), y8, mean, torch.full((n,), 2.0 ** -20, device="cuda"))
+    assert torch.isfinite(dx).all() and torch.equal(dgamma.double(), n * 2.0 ** -20 * U.load(q, e)[0]) and (dbeta == n).all()
