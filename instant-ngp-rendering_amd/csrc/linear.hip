@@ -698,7 +698,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_rows(const T* __restrict__ 
 // workgroups of four waves take ROWS rows at a time: dz and the layer's input go to LDS in 16 bits ([row][feature], from
 // where dx reads dz along its rows and dW reads both transposed), the weights' fragments and the workgroup's share of dW stay
 // in registers, the next rows are on their way from memory meanwhile.  dW and db leave as a share per workgroup.
-// 64 -> 64 over 2^18 rows moves 134 MB instead of the 233 MB of separate passes: 33 us (4.1 TB/s), and 5 to join the shares.
+// 64 -> 64 over 2^18 rows moves 134 MB instead of the 233 MB of separate passes: 30..33 us (4.1..4.5 TB/s), and 5 to join the
+// shares.  The registers' bound is the grid's two workgroups per CU (one for 128 x 128): pressed into a third's, the odd
+// widths' 195 registers spill (45 -> 61: 84 us and 60; the even ones' 168 fit either way, 30 us).  Of 64 / 128 the odd 64 -> 128
+// still spills 47 (bf16) or 65 registers under the bound of two (45 -> 91: 111 us; 64 -> 128: 43), the even forms 2 and 10.
 template <class T>
 struct NarrowArgs {
 	Kept<T> dy, z, x;
@@ -713,7 +716,7 @@ struct NarrowArgs {
 };
 
 template <class T, int NI, int NO, bool EVEN>
-__global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : NI + NO > 128 ? 2 : 3) k_narrow_backward(NarrowArgs<T> a) {
+__global__ void __launch_bounds__(256, NI + NO > 192 ? 1 : 2) k_narrow_backward(NarrowArgs<T> a) {
 	constexpr int ROWS = 64;
 	constexpr int DZ_ITEMS = ROWS * NO / 8 / 256, X_ITEMS = ROWS * NI / 8 / 256;  // eights per thread
 	constexpr int STRIPS = ROWS / 32, NT = NI / 32 / (4 / STRIPS);               // a wave's strip of dx: NT tiles of 32 columns

@@ -1,6 +1,13 @@
-"""What the compiler has to be told about the layer kernels' inline assembly, on the CPU."""
+"""What the compiler has to be told about the layer kernels, and what it made of them, on the CPU."""
 import os
 import re
+import shutil
+import struct
+import subprocess
+
+import pytest
+
+import ngp_abi
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "instant-ngp-rendering_amd", "csrc")
 
@@ -18,3 +25,37 @@ def test_inline_assembly_names_what_it_writes():
             clobbers = block.split(":")[-1]
             assert '"m0"' in clobbers and '"memory"' in clobbers, (name, block)
     assert found == 1
+
+
+def device_code(path):
+    """The gfx950 code objects in a library, one per source."""
+    with open(path, "rb") as f:
+        data = f.read()
+    magic, at, out = b"__CLANG_OFFLOAD_BUNDLE__", 0, []
+    while (at := data.find(magic, at)) >= 0:
+        count, = struct.unpack_from("<Q", data, at + len(magic))
+        p = at + len(magic) + 8
+        for _ in range(count):
+            offset, size, length = struct.unpack_from("<QQQ", data, p)
+            if data[p + 24:p + 24 + length].endswith(b"gfx950"):
+                out.append(data[at + offset:at + offset + size])
+            p += 24 + length
+        at += len(magic)
+    return out
+
+
+def test_the_one_pass_backward_of_64_wide_layers_keeps_its_registers(tmp_path):
+    """Even widths and odd: a bound for more workgroups than the grid has would make them spill."""
+    readelf = shutil.which("llvm-readelf") or "/opt/rocm/llvm/bin/llvm-readelf"
+    if not os.path.exists(readelf) or not os.path.exists(ngp_abi.LIB_PATH):
+        pytest.skip("needs the built library and llvm-readelf")
+    found = {}
+    for k, code in enumerate(device_code(ngp_abi.LIB_PATH)):
+        (tmp_path / f"{k}.co").write_bytes(code)
+        notes = subprocess.run([readelf, "--notes", str(tmp_path / f"{k}.co")], capture_output=True, text=True, check=True).stdout
+        for entry in notes.split("- .agpr_count:")[1:]:
+            symbol = re.search(r"\.symbol: +'?(\S+?)(\.kd)?'?\n", entry)
+            found[symbol.group(1)] = int(re.search(r"\.vgpr_spill_count: +(\d+)", entry).group(1))
+    kernels = {k: v for k, v in found.items() if "k_narrow_backward" in k and "Li64ELi64E" in k}
+    assert len(kernels) == 4, sorted(found)
+    assert not any(kernels.values()), kernels
