@@ -135,13 +135,15 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 3) k_norm_backwar
 			x.widen8(raw[c], xv);
 #pragma unroll
 			for (int k = 0; k < 8; ++k) {
-				const float d = widen(dy[c][k]), xh = (xv[k] - mean) * rstd, e = d * gamma[c][k];  // d is 0 past the row
+				// past the row d and x are 0: 0 times -mean is 0, where times rstd it might be infinite, so that is left for the sum
+				const float d = widen(dy[c][k]), centred = xv[k] - mean, e = d * gamma[c][k];
 				s[0] += e;
-				s[1] += e * xh;
-				if constexpr (SUMS) dg[c][k] += d * xh, db[c][k] += d;
+				s[1] += e * centred;
+				if constexpr (SUMS) dg[c][k] += d * (centred * rstd), db[c][k] += d;
 			}
 		}
 		if (!a.dx) continue;
+		s[1] *= rstd;
 		group_sums(s, G, lds + turn);
 		const float m0 = s[0] / (float)a.width, m1 = s[1] / (float)a.width;
 #pragma unroll
@@ -188,32 +190,33 @@ __global__ void __launch_bounds__(1024) k_norm_backward_rows(ngp_layer_norm_back
 	for (size_t i = blockIdx.x; i < a.n; i += gridDim.x, turn ^= 1u) {
 		const T* dy = static_cast<const T*>(a.dy) + i * a.dy_stride;
 		const float mean = a.mean[i], rstd = a.rstd[i];
-		auto chunk = [&](uint32_t j, float (&e)[8], float (&xh)[8]) {  // dy gamma and the normalised x
+		auto chunk = [&](uint32_t j, float (&e)[8], float (&centred)[8]) {  // dy gamma and x - mean: 0 and -mean past the row
 			const uint32_t left = a.width - j;
 			float gamma[8];
 #pragma unroll
 			for (int k = 0; k < 8; ++k) gamma[k] = 1.0f;
 			if (a.gamma) load8(a.gamma + j, left, gamma);
 			load8(dy + j, left, e);
-			x.at8(i, j, left, xh);
+			x.at8(i, j, left, centred);
 #pragma unroll
-			for (int k = 0; k < 8; ++k) e[k] *= gamma[k], xh[k] = (xh[k] - mean) * rstd;
+			for (int k = 0; k < 8; ++k) e[k] *= gamma[k], centred[k] -= mean;
 		};
-		float s[2] = {0.0f, 0.0f}, e[8], xh[8];
+		float s[2] = {0.0f, 0.0f}, e[8], centred[8];
 		for (uint32_t j = threadIdx.x * 8u; j < a.width; j += 8192u) {
-			chunk(j, e, xh);
+			chunk(j, e, centred);
 #pragma unroll
-			for (int k = 0; k < 8; ++k) s[0] += e[k], s[1] += e[k] * xh[k];
+			for (int k = 0; k < 8; ++k) s[0] += e[k], s[1] += e[k] * centred[k];
 		}
+		s[1] *= rstd;
 		group_sums(s, 1024u, part[turn]);
 		s[0] /= (float)a.width;
 		s[1] /= (float)a.width;
 		for (uint32_t j = threadIdx.x * 8u; j < a.width; j += 8192u) {
-			chunk(j, e, xh);
+			chunk(j, e, centred);
 			float add[8] = {};
 			if (a.dx_add) load8(static_cast<const T*>(a.dx_add) + i * a.dx_add_stride + j, a.width - j, add);
 #pragma unroll
-			for (int k = 0; k < 8; ++k) e[k] = rstd * (e[k] - s[0] - xh[k] * s[1]) + add[k];
+			for (int k = 0; k < 8; ++k) e[k] = rstd * (e[k] - s[0] - centred[k] * rstd * s[1]) + add[k];
 			store8(static_cast<T*>(a.dx) + i * a.dx_stride + j, a.width - j, e);
 		}
 	}

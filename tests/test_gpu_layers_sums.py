@@ -130,3 +130,20 @@ def test_norms_keep_rows_that_are_not_finite_to_themselves(n, width, kind):
         assert not torch.isfinite(dx[at]).any() and torch.equal(dx[keep], back[0][keep])
         assert not torch.isfinite(dg[3]) and not torch.isfinite(db[3])
         assert torch.equal(dg[cols != 3], back[1][cols != 3]) and torch.equal(db[cols != 3], back[2][cols != 3])
+
+
+# what lies past a row's end is no part of its sums: not where a row's mean times rstd leaves fp32's range either (equal values,
+# whose rstd is epsilon's alone).  With x = mean the formula is dx = rstd (g - mean(g)) + add.
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n, width", [(1, 1), (5, 8), (3, 33), (300, 40), (4000, 100), (70, 777), (5, 4100), (3, 9001), (2500, 9001)])
+def test_norm_backward_of_equal_large_values(n, width, kind):
+    t = U.TYPES[kind][1]
+    x, dy, add = torch.full((n, width), 2.0 ** 120, device="cuda").to(t), small(1, n, width, t=t), small(2, n, width, t=t)
+    mean, rstd = torch.full((n,), 2.0 ** 120, device="cuda"), torch.full((n,), 1024.0, device="cuda")
+    dx, dgamma, dbeta = U.call_layer_norm_backward(kind, dy, x, mean, rstd, add=add)
+    want = 1024.0 * (dy.double() - dy.double().mean(-1, keepdim=True)) + add.double()
+    tol = 1024.0 * 4 * 2.0 ** -23 * 3 + want.abs() * 2 * torch.finfo(t).eps  # sums of whole numbers, one quotient, a few roundings
+    assert ((dx.double() - want).abs() <= tol).all()
+    assert (dgamma == 0).all()
+    equal(dbeta, dy.sum(0, dtype=torch.float64), "dbeta")
+    assert torch.equal(U.call_layer_norm_backward(kind, dy, U.call_store(kind, x), mean, rstd, add=add)[0], dx)
