@@ -4,7 +4,8 @@
 // x (or its checkpoint) and the other branch's gradient and writes dx.  So every value is read once and stays in registers:
 // a row belongs to a group of G threads (4 .. 1024, a power of two), each of which holds up to C chunks of eight
 // neighbouring features, chunk c of thread g at features 8 (c G + g).  Groups of up to a wave sum with lane exchanges
-// alone, larger ones through LDS.
+// alone, larger ones through LDS.  (Only fp32 rows over 32768 values, eight chunks in each of 1024 threads, are more than a
+// thread's 128 registers hold: 6 of them spill.)
 #include <algorithm>
 
 #include "layer_math.h"
@@ -278,8 +279,8 @@ static void norm_forward(const ngp_layer_norm_args& a, hipStream_t s) {
 }
 
 // Backward: a quarter of the chunks, since a thread keeps two sums per column.  As many workgroups per CU as their registers
-// allow, three of 256 or (rows over 4096) one of 512, go through the rows in turns (65536 rows of 2048 fp16: 201 us, with two
-// per CU 220, with four chunks per thread 266; 20000 rows of 6000 with four chunks of 256 threads 327 us).
+// allow, three of 256 or (rows over 4096) one of 512, go through the rows in turns (65536 rows of 2048 fp16, in turn on one
+// box: 214..217 us, with two per CU 232..241, with two and four chunks per thread 313..319).
 constexpr uint32_t NORM_IN_PASS = 512 * 2 * 8;
 struct NormBackwardPlan {
 	NormShape shape;

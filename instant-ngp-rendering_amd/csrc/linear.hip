@@ -498,10 +498,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(Produc
 // 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
 // reads its next fragments and asks for a stage of K ahead, and then they change places.  A barrier after each half keeps
 // the two sets of four waves in opposite phases.  K goes through 128 KiB of LDS in stages of DEEP, each multiplied in steps
-// of 32: two buffers of 64 or four of 32.  Measured over 16384 rows of 2048 x 8192 (0.55 TFLOP, bf16): dW
-// 455 us (1.2 PFLOP/s, the matrix cores busy for 72 % of the cycles at the clock that they then run at), y and dx 595 us, of
-// which about 0.14 ms are the epilogues, which have the CU to themselves: with a gelu and a checkpoint 28 instructions per value,
-// 95 us of them, and 3 bytes written, 80 us (a 28th fewer instructions changed nothing for y and 1 % for dx).
+// of 32: two buffers of 64 or four of 32.  Measured over 16384 rows of 2048 x 8192 (0.55 TFLOP, bf16; by box): dW
+// 435..465 us (1.2 PFLOP/s, the matrix cores busy for 72 % of the CUs' busy cycles), y 575..615 and dx 570..625 us (busy for
+// 51 %), of which about 0.14 ms are the epilogues, which have the CU to themselves: with a gelu and a checkpoint 28 instructions
+// per value and 3 bytes written (with neither y is 55 us shorter).
 template <class T, class Out, bool P_BY_K, bool Q_BY_K, int DEEP>
 __global__ void __launch_bounds__(WIDE_THREADS, 2) k_product_wide(ProductArgs a, Out out) {
 	constexpr int TILE = 256, TM = 4, TN = 2, BUFFERS = 128 / DEEP;
@@ -1028,7 +1028,9 @@ struct ProductPlan {
 // rounded up, a stage of 64 k takes max(least, n each): a 64 tile's loads and barriers take as long as two of it multiply
 // (1024^3: 8 us with 64 tiles, 12 with 128, 25 with 256), a 256 tile moves a quarter of the bytes per multiplication (4096 x
 // 2048 x 4096: 105, 70 and 60 us).  Splits write their sums and read them again at about 4.2 TB/s, in a launch of their own
-// (32 x 4096 x 4096: 19 us with 64 tiles, 12 with four splits; 2048 x 1024 x 1024: 10 us, 24 with two).
+// (32 x 4096 x 4096: 19 us with 64 tiles, 12 with four splits; 2048 x 1024 x 1024: 10 us, 24 with two).  Each product is taken
+// as if it had the GPU to itself: dx and dW side by side share it and take longer together than either estimate says (3001 rows
+// 777 -> 1030: 15 us estimated for each, 31 measured for both).
 static ProductPlan plan_product(size_t M, uint32_t N, size_t K, int only = 0) {
 	struct Kind {
 		int tile;
@@ -1091,8 +1093,9 @@ static bool is_short(const ProductPlan& plan) { return plan.k_each <= 2 * PRODUC
 template <class T, class Out, bool P_BY_K, bool Q_BY_K>
 static void product(const ProductPlan& plan, const ProductArgs& a, const Out& out, hipStream_t s) {
 	const uint32_t blocks = a.tiles_m * a.tiles_n * a.splits;
-	// (rows along k come 128 bytes at a time from stages of 64: half the requests to L2, y of 16384 x 2048 x 8192 666 us, 704 with
-	// stages of 32; with an operand by k, whose lines are long either way, stages of 32 ask further ahead: dx 655 us, 673)
+	// (rows along k come 128 bytes at a time from stages of 64: half the requests to L2, y of 16384 x 2048 x 8192 578 us, 603 with
+	// stages of 32; with an operand by k, whose lines are long either way, stages of 32 ask further ahead: dx 260 M busy cycles,
+	// 278 M with stages of 64 (574 us and 580); dW alone would have the stages of 64, 423 us and 436)
 	if (plan.tile == 256) launch_lds(k_product_wide<T, Out, P_BY_K, Q_BY_K, P_BY_K || Q_BY_K ? 32 : 64>, blocks, WIDE_THREADS, 131072, s, a, out);
 	else if (plan.tile == 128) launch_lds(k_product<T, Out, P_BY_K, Q_BY_K, 128, 2>, blocks, PRODUCT_THREADS, 2 * 32768, s, a, out);
 	else if (is_short(plan)) launch_lds(k_product<T, Out, P_BY_K, Q_BY_K, 64, 2>, blocks, PRODUCT_THREADS, 2 * 16384, s, a, out);
