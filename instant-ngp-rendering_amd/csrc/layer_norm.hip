@@ -280,7 +280,7 @@ static void norm_forward(const ngp_layer_norm_args& a, hipStream_t s) {
 
 // Backward: a quarter of the chunks, since a thread keeps two sums per column.  As many workgroups per CU as their registers
 // allow, three of 256 or (rows over 4096) one of 512, go through the rows in turns (65536 rows of 2048 fp16, in turn on one
-// box: 214..217 us, with two per CU 232..241, with two and four chunks per thread 313..319).
+// card: 214..217 us, with two per CU 232..241, with two and four chunks per thread 313..319).
 constexpr uint32_t NORM_IN_PASS = 512 * 2 * 8;
 struct NormBackwardPlan {
 	NormShape shape;

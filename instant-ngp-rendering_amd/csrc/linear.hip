@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 2) k_backward_products(Produc
 // 256 x 256 of C per workgroup of eight waves, two by four, two waves to a SIMD: while the one of them multiplies, the other
 // reads its next fragments and asks for a stage of K ahead, and then they change places.  A barrier after each half keeps
 // the two sets of four waves in opposite phases.  K goes through 128 KiB of LDS in stages of DEEP, each multiplied in steps
-// of 32: two buffers of 64 or four of 32.  Measured over 16384 rows of 2048 x 8192 (0.55 TFLOP, bf16; by box): dW
+// of 32: two buffers of 64 or four of 32.  Measured over 16384 rows of 2048 x 8192 (0.55 TFLOP, bf16; by card): dW
 // 435..465 us (1.2 PFLOP/s, the matrix cores busy for 72 % of the CUs' busy cycles), y 575..615 and dx 570..625 us (busy for
 // 51 %), of which about 0.14 ms are the epilogues, which have the CU to themselves: with a gelu and a checkpoint 28 instructions
 // per value and 3 bytes written (with neither y is 55 us shorter).
